@@ -1,13 +1,17 @@
 """Embedding gather / scatter-add (vocab-parallel aware).
 
-Reference parity: src/layers.py:788-900 (F.embedding). The backward
-accumulates in fp32 with atomics, into ``weight.main_grad`` when the weight
-has one.
+Reference parity: src/layers.py:788-900 (F.embedding). The backward of
+``embedding`` accumulates in fp32 with atomics, into ``weight.main_grad`` when
+the weight has one. ``scaled_embedding`` multiplies the rows by a constant and
+sums its weight gradient over tokens sorted by id: the same bits every time,
+and the gradient is written in its own type in one pass instead of through an
+fp32 copy.
 """
 from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from ._ext import ext
 
@@ -45,3 +49,57 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, vocab_start: int = 0) -> 
     mask = (local < 0) | (local >= weight.shape[0])
     out = F.embedding(local.clamp(0, weight.shape[0] - 1), weight)
     return out.masked_fill(mask[..., None], 0.0)
+
+
+class _ScaledEmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, vstart):
+        ctx.save_for_backward(ids)
+        ctx.meta = (weight, scale, vstart)
+        return ext().scaled_embedding_fwd(ids, weight.contiguous(), scale, vstart)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        (ids,) = ctx.saved_tensors
+        weight, scale, vstart = ctx.meta
+        ids, dout = ids.reshape(-1), dout.reshape(-1, weight.shape[1]).contiguous()
+        mg = getattr(weight, "main_grad", None)
+        if mg is None:
+            dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+            ext().scaled_embedding_bwd(ids, dout, scale, vstart, dw, False)
+            return None, dw, None, None
+        ext().scaled_embedding_bwd(ids, dout, scale, vstart, mg, True)
+        hook = getattr(weight, "_ntb_grad_ready_hook", None)
+        if hook is not None:
+            hook(weight)
+        return None, None, None, None
+
+
+def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, *,
+                     vocab_start: int = 0) -> torch.Tensor:
+    """``scale`` times the rows of ``weight`` for ``ids``; ids outside [vocab_start, vocab_start + V) give zeros.
+
+    ids [...] (int64), weight [V, H] (bf16 or fp32 on CUDA, any floating type on the CPU); returns [..., H] in the
+    weight's type, rounded once. The gradient of ``weight`` is summed in fp32 over the tokens sorted by id, in their
+    order, and rounded once; with an fp32 ``main_grad`` on the weight it is added there instead.
+    """
+    if weight.dim() != 2:
+        raise ValueError(f"scaled_embedding: weight [V, H] expected, got {tuple(weight.shape)}")
+    if ids.dtype != torch.int64:
+        raise TypeError(f"scaled_embedding: ids must be int64, got {ids.dtype}")
+    if ids.device != weight.device:
+        raise ValueError(f"scaled_embedding: ids on {ids.device}, weight on {weight.device}")
+    if weight.is_cuda:
+        if weight.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"scaled_embedding: CUDA weights must be bfloat16 or float32, got {weight.dtype}")
+        return _ScaledEmbeddingFn.apply(ids.contiguous(), weight, float(scale), vocab_start)
+    if not weight.dtype.is_floating_point:
+        raise TypeError(f"scaled_embedding: floating weight expected, got {weight.dtype}")
+    local = ids - vocab_start
+    outside = (local < 0) | (local >= weight.shape[0])
+    if weight.shape[0] == 0:
+        return weight.new_zeros(*ids.shape, weight.shape[1])
+    rows = F.embedding(local.masked_fill(outside, 0), weight)
+    wide = rows if rows.dtype == torch.float64 else rows.float()
+    return (wide * scale).to(weight.dtype).masked_fill(outside[..., None], 0.0)

@@ -1,0 +1,289 @@
+"""The language-model head with its loss, without materialised logits.
+
+``linear_cross_entropy(hidden, weight, labels)`` is ``cross_entropy(linear(hidden, weight), labels)`` and
+``linear_distillation(hidden, weight, values, indices)`` the divergence from a teacher's top logits, each with its
+gradients. The [T, V] logits exist as 16-bit pieces of at most ``max_workspace_mb`` inside one call (on a chunk of
+tokens at a time) and never afterwards; statistics and losses come from the fp32 accumulators of the head's GEMM,
+so no 16-bit rounding of the logits enters the loss. Tokens without a target are taken out before the first GEMM:
+they cost no head FLOPs and reach no gradient, whatever they hold.
+
+For ``reduction="mean"`` and ``"sum"`` the gradients are computed with the loss (6 T V H operations in all) and the
+backward pass only scales them by the upstream gradient. ``"none"`` and vocabulary shards (``group``) need numbers
+that only the backward pass or the other ranks have: there the head's GEMM runs again in the backward pass
+(8 T V H). A second backward pass through the same graph does the same.
+
+CUDA tensors are bf16 (the operand type of the tensor-core GEMM), with 32-bit sums; CPU tensors of any floating
+type run the PyTorch formulation. When the weight carries an fp32 ``main_grad``, its gradient is added there and
+autograd receives none, as for the linears.
+
+Reference parity: src/losses.py:95-133 on the logits of src/models/transformer.py:25-289 (the reference keeps the
+logits); distillation has no counterpart there.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.distributed as dist
+from torch.autograd.function import once_differentiable
+
+from ._ext import ext
+
+_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
+DEFAULT_WORKSPACE_MB = 2048
+MAX_TEACHER_LOGITS = 1024
+
+
+def _grad_buffer(weight) -> Optional[torch.Tensor]:
+    mg = getattr(weight, "main_grad", None)
+    return mg if mg is not None and mg.dtype == torch.float32 and mg.is_cuda and mg.is_contiguous() else None
+
+
+def _deliver_weight_grad(weight, dw, factor=None):
+    """dw (times a device scalar) into ``main_grad`` when the weight has one, else as the weight's gradient."""
+    if dw is None:
+        return None
+    mg = getattr(weight, "main_grad", None)
+    if mg is not None:
+        into = _grad_buffer(weight)
+        if into is not None and dw.dtype == torch.float32:
+            ext().head_scaled_copy_(dw, factor, into, True)
+        else:
+            mg.add_(dw if factor is None else dw * factor)
+        hook = getattr(weight, "_ntb_grad_ready_hook", None)
+        if hook is not None:
+            hook(weight)
+        return None
+    if dw.dtype == weight.dtype:
+        if factor is not None:
+            ext().head_scale_(dw, factor)
+        return dw
+    out = torch.empty_like(dw, dtype=weight.dtype)
+    ext().head_scaled_copy_(dw, factor, out, False)
+    return out
+
+
+def _world(group) -> int:
+    return dist.get_world_size(group) if group is not None else 1
+
+
+class _HeadLossFn(torch.autograd.Function):
+    """Loss of a head over compacted tokens; ``labels`` or (``values``, ``indices``) are its targets."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, labels, values, indices, tau, ignore_index, reduction, vstart, group, nbytes,
+                with_grad):
+        shape = hidden.shape
+        h = _rows_operand(hidden.reshape(-1, shape[-1]))
+        w = _rows_operand(weight)
+        sharded = _world(group) > 1
+        need_dh = with_grad and ctx.needs_input_grad[0]
+        need_dw = with_grad and ctx.needs_input_grad[1]
+        now = reduction != "none" and not sharded and (need_dh or need_dw)
+        red = _REDUCTIONS["none" if sharded else reduction]
+        dw_f32 = getattr(weight, "main_grad", None) is not None
+        if labels is not None:
+            out = ext().linear_ce_fwd(h, w, labels, vstart, ignore_index, red, now and need_dh, now and need_dw, dw_f32,
+                                      nbytes)
+        else:
+            out = ext().linear_distill_fwd(h, w, values, indices, tau, red, now and need_dh, now and need_dw, dw_f32,
+                                           nbytes)
+        loss, lse2, picked, targets, tmap, place, count, q, _constant, dh, dw = out
+        if sharded:
+            loss, lse2 = _join_shards(loss, lse2, picked, targets, tmap, count, reduction, group)
+        if with_grad:
+            ctx.save_for_backward(h, w, lse2, picked, targets, tmap, place, count, q)
+            ctx.ready = (dh, dw) if now else None
+            ctx.meta = (weight, shape, tau, reduction, group if sharded else None, nbytes, dw_f32)
+        return loss.view(shape[:-1]) if reduction == "none" else loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        weight, shape, tau, reduction, group, nbytes, dw_f32 = ctx.meta
+        need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        gout = gout.float()
+        none = (None,) * 10
+        if ctx.ready is not None:
+            dh, dw = ctx.ready
+            ctx.ready = None  # handed on: a second backward pass computes them again
+            factor = gout.reshape(1)
+            if dh is not None:
+                ext().head_scale_(dh, factor)
+                dh = dh.view(shape)
+            return (dh, _deliver_weight_grad(weight, dw, factor), *none)
+        h, w, lse2, picked, targets, tmap, place, count, q = ctx.saved_tensors
+        if reduction == "none":
+            scale = gout.reshape(-1).contiguous()
+        else:
+            if reduction == "mean":
+                gout = gout / count.clamp_min(1)
+            scale = gout.reshape(1).expand(h.shape[0]).contiguous()
+        dh, dw = ext().linear_head_bwd(h, w, lse2, picked, targets, tmap, place, count, q, scale, tau, need_dh, need_dw,
+                                       dw_f32, nbytes)
+        if dh is not None:
+            if group is not None:
+                dist.all_reduce(dh, group=group)
+            dh = dh.view(shape)
+        return (dh, _deliver_weight_grad(weight, dw), *none)
+
+
+def _rows_operand(t: torch.Tensor) -> torch.Tensor:
+    """A 2-D view the tensor maps take: unit inner stride, every row on a 16-byte boundary."""
+    if t.stride(-1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) and t.stride(0) % 8 == 0 \
+            and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _join_shards(rows, lse2, picked, targets, tmap, count, reduction, group):
+    """Row losses over a vocabulary sharded across ``group``: lse and the label's logit are summed over the ranks.
+
+    ``rows`` is each rank's loss with the logits it has; log-sum-exp joins by (MAX, SUM), the label's logit, which
+    one rank has, by SUM. Statistics are in compact token order; rows past the device count are not read.
+    """
+    T = rows.numel()
+    live = torch.arange(T, device=rows.device) < count
+    lse2 = torch.where(live, lse2, 0.0)
+    tok = torch.where(live, tmap[:T].long(), 0)
+    here = live & (targets.view(-1)[tok] != torch.iinfo(torch.int32).max)
+    x2 = torch.where(here, picked[:, 0], 0.0)
+    top = lse2.clone()
+    dist.all_reduce(top, op=dist.ReduceOp.MAX, group=group)
+    total = torch.exp2(lse2 - top)
+    dist.all_reduce(total, group=group)
+    dist.all_reduce(x2, group=group)
+    lse2 = top + torch.log2(total)
+    value = torch.where(live, (lse2 - x2) * 0.6931471805599453, 0.0)
+    loss = torch.zeros_like(rows).index_add_(0, tok, value)
+    if reduction == "none":
+        return loss, lse2
+    loss = loss.sum()
+    return (loss / count[0].clamp_min(1) if reduction == "mean" else loss), lse2
+
+
+def _check(name, hidden, weight, reduction, max_workspace_mb):
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{name}: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{name}: hidden [..., H] and weight [V, H] disagree: {tuple(hidden.shape)}, "
+                         f"{tuple(weight.shape)}")
+    if weight.shape[0] < 1:
+        raise ValueError(f"{name}: empty vocabulary")
+    if hidden.dtype != weight.dtype or not hidden.dtype.is_floating_point:
+        raise TypeError(f"{name}: hidden and weight must have one floating dtype, got {hidden.dtype}, {weight.dtype}")
+    if hidden.device != weight.device:
+        raise ValueError(f"{name}: hidden on {hidden.device}, weight on {weight.device}")
+    if max_workspace_mb <= 0:
+        raise ValueError(f"{name}: max_workspace_mb must be positive")
+    if hidden.is_cuda:
+        if hidden.dtype != torch.bfloat16:
+            raise TypeError(f"{name}: CUDA tensors must be bfloat16, got {hidden.dtype}")
+        if hidden.shape[-1] == 0 or hidden.shape[-1] % 8:
+            raise ValueError(f"{name}: the hidden size must be a multiple of 8 on CUDA, got {hidden.shape[-1]}")
+
+
+def _reduce(rows, valid, reduction):
+    if reduction == "none":
+        return rows
+    total = rows.sum()
+    return total if reduction == "sum" else total / valid.sum().clamp_min(1).to(total.dtype)
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
+                         reduction: str = "mean", *, vocab_start: int = 0, group=None,
+                         max_workspace_mb: int = DEFAULT_WORKSPACE_MB) -> torch.Tensor:
+    """Cross-entropy of the head ``hidden @ weight.T`` against ``labels``, without materialised logits.
+
+    hidden [..., H], weight [V, H], labels [...] (int64). Returns an fp32 scalar, or fp32 losses of the labels'
+    shape for ``reduction="none"`` (0 where the label is ``ignore_index``); the mean is over the other labels,
+    0 if there are none. With ``group``, ``weight`` holds rows [vocab_start, vocab_start + V) of a vocabulary
+    sharded over that group (``hidden`` and ``labels`` are the same on its ranks) and the gradient of ``hidden``
+    is summed over it. Without one, labels must be ``ignore_index`` or in [vocab_start, vocab_start + V).
+    """
+    _check("linear_cross_entropy", hidden, weight, reduction, max_workspace_mb)
+    if labels.dtype != torch.int64:
+        raise TypeError(f"linear_cross_entropy: labels must be int64, got {labels.dtype}")
+    if labels.shape != hidden.shape[:-1]:
+        raise ValueError(f"linear_cross_entropy: labels {tuple(labels.shape)} for hidden {tuple(hidden.shape)}")
+    if labels.device != hidden.device:
+        raise ValueError(f"linear_cross_entropy: labels on {labels.device}, hidden on {hidden.device}")
+    if hidden.is_cuda:
+        with_grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+        return _HeadLossFn.apply(hidden, weight, labels.reshape(-1).contiguous(), None, None, 1.0, ignore_index,
+                                 reduction, vocab_start, group, max_workspace_mb << 20, with_grad)
+    lab = labels.reshape(-1)
+    valid = lab != ignore_index
+    h = torch.where(valid[:, None], hidden.reshape(-1, hidden.shape[-1]), 0.0)
+    if _world(group) > 1:
+        from ..parallel.comm import copy_to_tensor_parallel_region
+        from .loss import _vocab_parallel_ce_reference
+
+        h = copy_to_tensor_parallel_region(h, group)
+        logits = h.float() @ weight.float().t()
+        out = _vocab_parallel_ce_reference(logits, lab, ignore_index, reduction, vocab_start, group)
+        return out.view(labels.shape) if reduction == "none" else out
+    logits = _wide(h) @ _wide(weight).t()
+    local = lab - vocab_start
+    inside = valid & (local >= 0) & (local < weight.shape[0])
+    target = logits.gather(1, torch.where(inside, local, 0)[:, None])[:, 0]
+    rows = torch.logsumexp(logits, 1) - torch.where(inside, target, 0.0)
+    rows = torch.where(valid, rows, 0.0)
+    return _reduce(rows.view(labels.shape), valid, reduction)
+
+
+def _wide(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_values: torch.Tensor,
+                        teacher_indices: torch.Tensor, temperature: float = 1.0, reduction: str = "mean", *,
+                        max_workspace_mb: int = DEFAULT_WORKSPACE_MB) -> torch.Tensor:
+    """Divergence of the head ``hidden @ weight.T`` from a teacher's top-K logits, without materialised logits.
+
+    hidden [..., H], weight [V, H], teacher_values [..., K] (fp32, bf16 or fp16 logits; K up to 1024),
+    teacher_indices [..., K] (int64 or int32). For each token, with q = softmax(values / temperature) over its K
+    entries and p = softmax(hidden @ weight.T / temperature) over the vocabulary:
+
+        loss = temperature^2 * sum_k q_k (log q_k - log p[index_k])
+
+    (the factor keeps the gradients' size independent of the temperature). Entries whose index is outside [0, V)
+    or whose value is -inf are padding; a token with no other entry has loss 0, no gradient and no part in the
+    mean. An index that occurs more than once stands for the sum of its q. The teacher receives no gradient.
+    """
+    _check("linear_distillation", hidden, weight, reduction, max_workspace_mb)
+    lead = hidden.shape[:-1]
+    if teacher_values.shape != teacher_indices.shape or teacher_values.shape[:-1] != lead or \
+            teacher_values.dim() != hidden.dim():
+        raise ValueError(f"linear_distillation: teacher values {tuple(teacher_values.shape)} and indices "
+                         f"{tuple(teacher_indices.shape)} for hidden {tuple(hidden.shape)}")
+    K = teacher_values.shape[-1]
+    if not 1 <= K <= MAX_TEACHER_LOGITS:
+        raise ValueError(f"linear_distillation: 1 to {MAX_TEACHER_LOGITS} teacher logits a token, got {K}")
+    if teacher_indices.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"linear_distillation: indices must be int64 or int32, got {teacher_indices.dtype}")
+    if not teacher_values.dtype.is_floating_point:
+        raise TypeError(f"linear_distillation: teacher values must be floating, got {teacher_values.dtype}")
+    if not temperature > 0:
+        raise ValueError(f"linear_distillation: temperature must be positive, got {temperature}")
+    if teacher_values.device != hidden.device or teacher_indices.device != hidden.device:
+        raise ValueError("linear_distillation: the teacher's tensors must be on the hidden states' device")
+    values, indices = teacher_values.detach().reshape(-1, K), teacher_indices.reshape(-1, K)
+    if hidden.is_cuda:
+        if values.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise TypeError(f"linear_distillation: teacher values must be fp32, bf16 or fp16, got {values.dtype}")
+        with_grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+        values = values if values.stride(-1) == 1 else values.contiguous()
+        indices = indices if indices.stride(-1) == 1 else indices.contiguous()
+        return _HeadLossFn.apply(hidden, weight, None, values, indices, float(temperature), 0, reduction, 0, None,
+                                 max_workspace_mb << 20, with_grad)
+    there = (indices >= 0) & (indices < weight.shape[0]) & (values != float("-inf"))
+    valid = there.any(1)
+    h = torch.where(valid[:, None], hidden.reshape(-1, hidden.shape[-1]), 0.0)
+    logp = torch.log_softmax(_wide(h) @ _wide(weight).t() / temperature, 1)
+    # Tokens without entries take a softmax over zeros, whose result is not used.
+    score = torch.where(there, _wide(values) / temperature, float("-inf"))
+    logq = torch.log_softmax(torch.where(valid[:, None], score, 0.0), 1)
+    at = logp.gather(1, torch.where(there, indices, 0).long())
+    rows = torch.where(there, logq.exp() * (torch.where(there, logq, 0.0) - at), 0.0).sum(1) * temperature ** 2
+    return _reduce(rows.view(lead), valid, reduction)

@@ -1,0 +1,150 @@
+"""The head losses and the scaled embedding on the CPU: formulas, gradients against differences, refusals, shards."""
+import math
+import os
+
+import pytest
+import torch
+import torch.multiprocessing as mp
+import torch.nn.functional as F
+
+from conftest import free_port
+from nano_train_b200 import ops
+
+
+def _inputs(T=9, H=16, V=23, dtype=torch.float64, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(T, H, generator=g, dtype=dtype).requires_grad_(True)
+    w = torch.randn(V, H, generator=g, dtype=dtype).requires_grad_(True)
+    lab = torch.randint(0, V, (T,), generator=g)
+    lab[2::3] = -100
+    return h, w, lab
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_cross_entropy_is_linear_then_cross_entropy(reduction):
+    h, w, lab = _inputs()
+    got = ops.linear_cross_entropy(h, w, lab, reduction=reduction)
+    want = F.cross_entropy(h @ w.t(), lab, reduction=reduction)
+    torch.testing.assert_close(got, want, rtol=1e-12, atol=1e-12)
+    up = torch.randn_like(got)
+    for a, b in zip(torch.autograd.grad(got, (h, w), up), torch.autograd.grad(want, (h, w), up)):
+        torch.testing.assert_close(a, b, rtol=1e-11, atol=1e-12)
+
+
+def test_gradients_against_differences():
+    h, w, lab = _inputs(T=4, H=5, V=7)
+    idx = torch.tensor([[1, 3, 3], [0, -1, 6], [-1, -1, -1], [5, 4, 2]])
+    val = torch.randn(4, 3, dtype=torch.float64)
+    assert torch.autograd.gradcheck(lambda a, b: ops.linear_cross_entropy(a, b, lab), (h, w))
+    assert torch.autograd.gradcheck(
+        lambda a, b: ops.linear_distillation(a, b, val, idx, temperature=1.7, reduction="none"), (h, w))
+    assert torch.autograd.gradcheck(lambda b: ops.scaled_embedding(lab[:2], b, 2.5, vocab_start=1), (w,))
+
+
+def test_masked_tokens_and_empty_calls():
+    h, w, lab = _inputs()
+    with torch.no_grad():
+        h[2] = float("nan")
+    loss = ops.linear_cross_entropy(h, w, lab)
+    loss.backward()
+    assert torch.isfinite(loss) and torch.isfinite(h.grad).all() and torch.isfinite(w.grad).all()
+    assert ops.linear_cross_entropy(h, w, torch.full_like(lab, -100)).item() == 0.0
+    assert ops.linear_cross_entropy(h[:0], w, lab[:0]).item() == 0.0
+    none = torch.full((9, 2), -1)
+    assert ops.linear_distillation(h, w, torch.zeros(9, 2), none).item() == 0.0
+
+
+def test_distillation_formula():
+    h, w, _ = _inputs(seed=1)
+    V = w.shape[0]
+    logits = torch.randn(9, V, dtype=torch.float64)
+    val, idx = logits.topk(V, dim=1)  # all of the vocabulary: the whole divergence
+    for tau in (1.0, 2.0):
+        got = ops.linear_distillation(h, w, val, idx, temperature=tau)
+        want = F.kl_div(F.log_softmax(h @ w.t() / tau, 1), F.log_softmax(logits / tau, 1), reduction="batchmean",
+                        log_target=True) * tau * tau
+        torch.testing.assert_close(got, want, rtol=1e-11, atol=1e-12)
+    # entries outside the vocabulary and -inf values are padding
+    val2, idx2 = val[:, :4].clone(), idx[:, :4].clone()
+    idx2[:, 3] = V + 1
+    val2[:, 2] = -math.inf
+    torch.testing.assert_close(ops.linear_distillation(h, w, val2, idx2),
+                               ops.linear_distillation(h, w, val[:, :2], idx[:, :2]))
+
+
+def test_scaled_embedding_formula():
+    w = torch.randn(6, 5, requires_grad=True)
+    ids = torch.tensor([[0, 3], [7, 3]])
+    out = ops.scaled_embedding(ids, w, 2.0, vocab_start=1)
+    torch.testing.assert_close(out, torch.stack([torch.zeros(5), 2 * w[2], torch.zeros(5), 2 * w[2]]).view(2, 2, 5))
+    out.sum().backward()
+    want = torch.zeros(6, 5)
+    want[2] = 4.0
+    torch.testing.assert_close(w.grad, want)
+
+
+def test_refusals():
+    h, w, lab = _inputs(dtype=torch.float32)
+    with pytest.raises(ValueError):
+        ops.linear_cross_entropy(h, w, lab, reduction="max")
+    with pytest.raises(ValueError):
+        ops.linear_cross_entropy(h, w[:, :8], lab)
+    with pytest.raises(TypeError):
+        ops.linear_cross_entropy(h, w.double(), lab)
+    with pytest.raises(TypeError):
+        ops.linear_cross_entropy(h, w, lab.int())
+    with pytest.raises(ValueError):
+        ops.linear_cross_entropy(h, w, lab[:4])
+    with pytest.raises(ValueError):
+        ops.linear_cross_entropy(h, w[:0], lab)
+    with pytest.raises(ValueError):
+        ops.linear_cross_entropy(h, w, lab, max_workspace_mb=0)
+    val, idx = torch.zeros(9, 3), torch.zeros(9, 3, dtype=torch.int64)
+    for bad in (0.0, -1.0, float("nan")):
+        with pytest.raises(ValueError):
+            ops.linear_distillation(h, w, val, idx, temperature=bad)
+    with pytest.raises(ValueError):
+        ops.linear_distillation(h, w, val, idx[:, :2])
+    with pytest.raises(ValueError):
+        ops.linear_distillation(h, w, val[:, :0], idx[:, :0])
+    with pytest.raises(TypeError):
+        ops.linear_distillation(h, w, val, idx.float())
+    with pytest.raises(TypeError):
+        ops.scaled_embedding(lab.int(), w)
+    with pytest.raises(ValueError):
+        ops.scaled_embedding(lab, w[0])
+
+
+def _shard_worker(rank, world, port, out):
+    import torch.distributed as dist
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        h, w, lab = _inputs(T=11, H=8, V=20, dtype=torch.float32)
+        V = w.shape[0] // world
+        res = {}
+        for reduction in ("mean", "none"):
+            a = h.detach().clone().requires_grad_(True)
+            b = w.detach()[rank * V:(rank + 1) * V].clone().requires_grad_(True)
+            loss = ops.linear_cross_entropy(a, b, lab, reduction=reduction, vocab_start=rank * V,
+                                            group=dist.group.WORLD)
+            loss.backward(torch.linspace(0.5, 1.5, 11) if reduction == "none" else None)
+            res[reduction] = (loss.detach(), a.grad, b.grad)
+        torch.save(res, f"{out}.{rank}")
+    finally:
+        dist.destroy_process_group()
+
+
+def test_cross_entropy_over_a_sharded_vocabulary(tmp_path):
+    out = str(tmp_path / "res")
+    mp.spawn(_shard_worker, args=(2, free_port(), out), nprocs=2, join=True)
+    h, w, lab = _inputs(T=11, H=8, V=20, dtype=torch.float32)
+    parts = [torch.load(f"{out}.{r}") for r in range(2)]
+    for reduction in ("mean", "none"):
+        loss = ops.linear_cross_entropy(h, w, lab, reduction=reduction)
+        up = torch.linspace(0.5, 1.5, 11) if reduction == "none" else torch.ones(())
+        dh, dw = torch.autograd.grad(loss, (h, w), up)
+        for p in parts:
+            torch.testing.assert_close(p[reduction][0], loss.detach(), rtol=1e-5, atol=1e-6)
+            torch.testing.assert_close(p[reduction][1], dh, rtol=1e-5, atol=1e-6)
+        torch.testing.assert_close(torch.cat([p[reduction][2] for p in parts]), dw, rtol=1e-5, atol=1e-6)

@@ -30,24 +30,23 @@ void gemm_bf16(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, const 
 void gemm_grouped_bf16(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, const at::Tensor& offsets,
                        int64_t mode, bool b_mn, bool accumulate, int64_t c_group_stride);
 // sorted_embedding.cu
-at::Tensor scaled_embedding_fwd(const at::Tensor& ids, const at::Tensor& W, double scale, int64_t vstart);
-void scaled_embedding_bwd(const at::Tensor& ids, const at::Tensor& dout, double scale, int64_t vstart, at::Tensor& dw,
-                          bool add);
+at::Tensor scaled_embedding(const at::Tensor& ids, const at::Tensor& weight, double scale, int64_t vstart);
+at::Tensor scaled_embedding_fwd(const at::Tensor& ids, const at::Tensor& weight, double scale, int64_t vstart);
+void scaled_embedding_add_(const at::Tensor& ids, const at::Tensor& dout, double scale, int64_t vstart, at::Tensor& dw);
 // vocab_head.cu
-std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& labels,
-                                      int64_t vstart, int64_t ignore_index, int64_t reduction, bool need_dh,
-                                      bool need_dw, bool dw_f32, int64_t bytes);
-std::vector<at::Tensor> linear_distill_fwd(const at::Tensor& hidden, const at::Tensor& weight,
-                                           const at::Tensor& values, const at::Tensor& indices, double tau,
-                                           int64_t reduction, bool need_dh, bool need_dw, bool dw_f32, int64_t bytes);
-std::vector<at::Tensor> linear_head_bwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& lse2,
-                                        const at::Tensor& picked, const at::Tensor& targets, const at::Tensor& map,
-                                        const at::Tensor& place, const at::Tensor& count,
-                                        const c10::optional<at::Tensor>& q, const at::Tensor& row_scale, double tau,
+at::Tensor linear_head_loss(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& a,
+                            const c10::optional<at::Tensor>& b, double tau, int64_t ignore_index, int64_t reduction,
+                            int64_t vstart, int64_t bytes);
+std::vector<at::Tensor> linear_head_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& a,
+                                        const c10::optional<at::Tensor>& b, double tau, int64_t ignore_index,
+                                        int64_t reduction, int64_t vstart, int64_t bytes, bool need_dh, bool need_dw,
+                                        bool dw_f32);
+std::vector<at::Tensor> linear_head_state(const at::Tensor& state, int64_t T, int64_t K, bool distill);
+std::vector<at::Tensor> linear_head_bwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& state,
+                                        int64_t K, bool distill, const at::Tensor& row_scale, double tau,
                                         bool need_dh, bool need_dw, bool dw_f32, int64_t bytes);
-void head_scale_(at::Tensor& x, const at::Tensor& factor);
-void head_scaled_copy_(const at::Tensor& src, const c10::optional<at::Tensor>& factor, at::Tensor& dst,
-                       bool accumulate);
+void linear_head_deliver_(const c10::optional<at::Tensor>& dh, const c10::optional<at::Tensor>& dw,
+                          const c10::optional<at::Tensor>& factor, const c10::optional<at::Tensor>& into);
 // ops.cu
 std::vector<at::Tensor> rmsnorm_fwd(const at::Tensor& x, const c10::optional<at::Tensor>& residual,
                                     const at::Tensor& w, double eps);
@@ -190,13 +189,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_grouped_bf16", &ntb::gemm_grouped_bf16, "grouped (mixture-of-experts) tcgen05 GEMM", py::arg("a"),
         py::arg("b"), py::arg("out"), py::arg("offsets"), py::arg("mode"), py::arg("b_mn") = false,
         py::arg("accumulate") = false, py::arg("c_group_stride") = 0);
+  m.def("scaled_embedding", &ntb::scaled_embedding, "scaled lookup, differentiable");
   m.def("scaled_embedding_fwd", &ntb::scaled_embedding_fwd);
-  m.def("scaled_embedding_bwd", &ntb::scaled_embedding_bwd, "weight gradient summed over tokens sorted by id");
-  m.def("linear_ce_fwd", &ntb::linear_ce_fwd, "linear head + cross-entropy in pieces, with its gradients");
-  m.def("linear_distill_fwd", &ntb::linear_distill_fwd, "linear head + distillation from a teacher's top logits");
-  m.def("linear_head_bwd", &ntb::linear_head_bwd, "linear head gradients with the statistics known");
-  m.def("head_scale_", &ntb::head_scale_);
-  m.def("head_scaled_copy_", &ntb::head_scaled_copy_);
+  m.def("scaled_embedding_add_", &ntb::scaled_embedding_add_, "fp32 dw += gradient summed over tokens sorted by id");
+  m.def("linear_head_loss", &ntb::linear_head_loss, "linear head + cross-entropy or distillation, differentiable");
+  m.def("linear_head_fwd", &ntb::linear_head_fwd);
+  m.def("linear_head_state", &ntb::linear_head_state);
+  m.def("linear_head_bwd", &ntb::linear_head_bwd);
+  m.def("linear_head_deliver_", &ntb::linear_head_deliver_);
   m.def("rmsnorm_fwd", &ntb::rmsnorm_fwd);
   m.def("rmsnorm_bwd", &ntb::rmsnorm_bwd, py::arg("dy"), py::arg("h"), py::arg("w"), py::arg("rstd"),
         py::arg("dres"), py::arg("dw_into") = py::none());

@@ -155,6 +155,7 @@ static void gemm_bf16_impl(const at::Tensor& a, const at::Tensor& b, at::Tensor&
     p.rows_base = tok->rows_base;
     p.rows_are_k = tok->rows_are_k ? 1 : 0;
     p.slice_stride = tok->slice_stride;
+    p.alpha_dev = tok->alpha_dev;
     if (tok->splits > 1) {
       TORCH_CHECK(p.c_f32 && !accumulate && tok->slice_stride >= M * p.ldc, "gemm_bf16: slices need their own fp32 rows");
       tc = {N > 128, tok->splits};
@@ -209,7 +210,7 @@ static void gemm_bf16_impl(const at::Tensor& a, const at::Tensor& b, at::Tensor&
 
 void gemm_bf16_tokens(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool a_mn, bool b_mn, bool accumulate,
                       const GemmTokenRows& tok) {
-  gemm_bf16_impl(a, b, out, c10::nullopt, a_mn, b_mn, accumulate, 1.0, {}, 0, nullptr, &tok);
+  gemm_bf16_impl(a, b, out, c10::nullopt, a_mn, b_mn, accumulate, tok.alpha, {}, 0, nullptr, &tok);
 }
 
 void gemm_bf16(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, const c10::optional<at::Tensor>& bias,

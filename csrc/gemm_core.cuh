@@ -43,6 +43,7 @@ struct GemmParams {
   const int* rows;
   int rows_base;
   int rows_are_k;
+  const float* alpha_dev;  // device factor of alpha (optional)
   // Publication (plain GEMM, optional): when pub_n > 0, the last CTA to finish makes the whole C
   // visible system-wide (fence.sc.sys) and stores pub_epoch into pub_flag[0..pub_n) - the epoch
   // words of the peers that read C over NVLink. pub_ctr: a device u32 that is zero at rest.
@@ -112,6 +113,7 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, float* stage, cons
   const bool f32 = p.c_f32 != 0;
   // red: a K-slice of a split GEMM (fp32 C) - the partial is added with atomics, C is not read.
   const bool acc = p.accumulate != 0 && !red;
+  const float alpha = p.alpha_dev != nullptr ? p.alpha * __ldg(p.alpha_dev) : p.alpha;
 #pragma unroll 1
   for (int g = 0; g < BN; g += 64) {
     const int cg = n0 + g;
@@ -151,7 +153,7 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, float* stage, cons
       for (int u = 0; u < 4; ++u) {
         const int c = j * 4 + u;
         const uint32_t bits = c < 32 ? r0[c] : r1[c - 32];
-        float x = __uint_as_float(bits) * p.alpha;
+        float x = __uint_as_float(bits) * alpha;
         if (p.bias != nullptr && !red && cg + c < p.N) x += __bfloat162float(p.bias[cg + c]);
         w[u] = x;
       }
@@ -268,14 +270,16 @@ __device__ __forceinline__ TileInfo tile_info(const GemmParams& p, int tile, int
 // What the epilogue warps do with an accumulator tile. An object lives for the whole kernel in each epilogue
 // thread: `begin` runs before the tile's accumulator is waited for (so it overlaps the main loop), `tile` with the
 // accumulator in TMEM. m0: first row of the warp's 32; n0: first column of the tile; Params derives from
-// GemmParams.
+// GemmParams; kWarps (4 or 8) warps share the 32 KB of staging. With 8, the second four take the tile's columns
+// from BN / 2 on (`part` 1).
 struct StoreEpilogue {
   using Params = GemmParams;
+  static constexpr int kWarps = 4;
   __device__ __forceinline__ StoreEpilogue(const Params&) {}
   __device__ __forceinline__ void begin(const Params&, long, int) {}
   template <int BN>
   __device__ __forceinline__ void tile(uint32_t t_row, float* stage, const Params& p, long m0, int n0, bool vec_ok,
-                                       long m_end, int slice) {
+                                       long m_end, int slice, int) {
     const bool split = p.splits > 1;
     epilogue_tile<BN>(t_row, stage, p, m0, n0, vec_ok, m_end, split && p.slice_stride == 0,
                       split ? slice * p.slice_stride : 0);
@@ -283,7 +287,7 @@ struct StoreEpilogue {
 };
 
 template <int BN, bool A_MN, bool B_MN, int GM = 0, class Epi = StoreEpilogue>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
     gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      typename Epi::Params p) {
   using Cfg = GemmCfg<BN>;
@@ -317,7 +321,7 @@ __global__ void __launch_bounds__(192, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 128);
+      mbar_init(&tempty[b], 32 * Epi::kWarps);
     }
     mbar_init(drain, 1);
     mbar_fence_init();
@@ -437,17 +441,18 @@ __global__ void __launch_bounds__(192, 1)
     int acc = 0;
     uint32_t acc_phase = 0;
     const bool vec_ok = ((p.ldc & 7) == 0) && ((reinterpret_cast<uintptr_t>(p.C) & 15) == 0);
-    float* stage = reinterpret_cast<float*>(stage_base + q * 8192);
+    const int epart = (warp - 2) >> 2;
+    float* stage = reinterpret_cast<float*>(stage_base + (epart * 4 + q) * (Cfg::STAGE_BYTES / Epi::kWarps));
     Epi epi(p);
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
       const TileInfo ti = tile_info<GM>(p, tile, num_m, num_n, num_kb, BM, BK);
       const long m0 = static_cast<long>(ti.mb) * BM + q * 32;
-      if constexpr (GM != 2) epi.begin(p, m0, ti.nb * BN);
+      if constexpr (GM != 2) epi.begin(p, m0, ti.nb * BN + epart * (BN / 2));
       if (!mbar_wait(&tfull[acc], acc_phase, p.status, kStatusTimeoutEpilogue)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
       if constexpr (GM != 2) {
-        epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, ti.slice);
+        epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, ti.slice, epart);
       } else if (ti.nkb > 0) {
         // Expert block: rows [group * M, group * M + M) of the stacked output; an expert without
         // rows contributes nothing (its accumulator was never written).
@@ -503,7 +508,7 @@ struct PairCfg {
 };
 
 template <bool A_MN, bool B_MN, class Epi = StoreEpilogue>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
     gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                           typename Epi::Params p) {
   using Cfg = PairCfg;
@@ -539,7 +544,7 @@ __global__ void __launch_bounds__(192, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 2 * 128);  // every epilogue thread of both CTAs
+      mbar_init(&tempty[b], 2 * 32 * Epi::kWarps);  // every epilogue thread of both CTAs
     }
     mbar_init(drain, 1);
     mbar_fence_init();
@@ -662,16 +667,17 @@ __global__ void __launch_bounds__(192, 1)
     int acc = 0;
     uint32_t acc_phase = 0;
     const bool vec_ok = ((p.ldc & 7) == 0) && ((reinterpret_cast<uintptr_t>(p.C) & 15) == 0);
-    float* stage = reinterpret_cast<float*>(stage_base + q * 8192);
+    const int epart = (warp - 2) >> 2;
+    float* stage = reinterpret_cast<float*>(stage_base + (epart * 4 + q) * (Cfg::STAGE_BYTES / Epi::kWarps));
     Epi epi(p);
     for (int tile = pair; tile < num_tiles; tile += npairs) {
       const TileInfo ti = tile_info<0>(p, tile, num_m, num_n, num_kb, 2 * BM, BK);
       const long m0 = static_cast<long>(ti.mb) * 2 * BM + rank * BM + q * 32;
-      epi.begin(p, m0, ti.nb * BN);
+      epi.begin(p, m0, ti.nb * BN + epart * (BN / 2));
       if (!mbar_wait(&tfull[acc], acc_phase, p.status, kStatusTimeoutEpilogue)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
-      epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, ti.slice);
+      epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, ti.slice, epart);
       tc_fence_before();
       mbar_arrive_cluster(tempty0 + 8u * static_cast<uint32_t>(acc));
       acc ^= 1;
@@ -714,7 +720,7 @@ static void launch_gemm(const CUtensorMap* ta, const CUtensorMap* tb, typename E
                         (GM == 2 ? p.groups : (GM == 0 && p.splits > 1 ? p.splits : 1));
   const int grid = std::min(num_tiles, num_sms(dev));
   void* args[3] = {const_cast<CUtensorMap*>(ta), const_cast<CUtensorMap*>(tb), &p};
-  NTB_CUDA_CHECK(cudaLaunchKernel(reinterpret_cast<const void*>(kern), dim3(grid), dim3(192), args,
+  NTB_CUDA_CHECK(cudaLaunchKernel(reinterpret_cast<const void*>(kern), dim3(grid), dim3(64 + 32 * Epi::kWarps), args,
                                   Cfg::SMEM_BYTES, stream));
   NTB_LAUNCH_CHECK(1);
 }
@@ -735,7 +741,7 @@ static void launch_gemm_pair(const CUtensorMap* ta, const CUtensorMap* tb, typen
   const int pairs = std::max(1, std::min(units, num_sms(dev) / 2));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * pairs);
-  cfg.blockDim = dim3(192);
+  cfg.blockDim = dim3(64 + 32 * Epi::kWarps);
   cfg.dynamicSmemBytes = PairCfg::SMEM_BYTES;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -69,6 +69,8 @@ struct GemmTokenRows {
   bool rows_are_k = false;
   int splits = 1;
   int64_t slice_stride = 0;
+  double alpha = 1.0;
+  const float* alpha_dev = nullptr;  // device factor of alpha
 };
 void gemm_bf16_tokens(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool a_mn, bool b_mn, bool accumulate,
                       const GemmTokenRows& tok);

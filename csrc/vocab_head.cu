@@ -12,24 +12,31 @@
 // tokens cost nothing and whatever they hold (NaN included) reaches no gradient.
 //
 // A chunk of tokens runs as
-//   1. logits GEMM (tcgen05, gemm_core.cuh) whose epilogue keeps, for each row and 256-column tile, the maximum m
+//   1. logits GEMM (tcgen05, gemm_core.cuh) whose epilogue keeps, for each row and 128-column tile, the maximum m
 //      and sum of 2^(x - m), picks the targets' logits out of the fp32 accumulators and writes the rest as 16-bit
 //      fixed-point distances (m - x) below the tile's maximum: steps of 2^-10 in base-2 units, an error of at most
 //      3.4e-4 of each probability (bf16 probabilities would have 3.9e-3), 64 powers of two deep;
 //   2. a row kernel that joins the tiles' statistics into lse, computes the row's loss and turns the distances in
-//      place into bf16 G, the targets' entries from their fp32 logits;
+//      place into bf16 p - q, the targets' entries from their fp32 logits;
 //   3. dH = G W, K (the vocabulary) cut into slices whose fp32 partials are added in a fixed order;
 //   4. dW (+)= G^T H.
 // That is 6 T V H operations, the least there is, at the price of a chunk of 16-bit G in memory. Where the
 // upstream gradient of each row is only known in the backward pass (per-token losses, a vocabulary sharded over
 // ranks), step 1 runs there a second time with lse known and writes G at once.
 //
-// Sums, statistics, losses and picked logits are fp32; G is rounded to bf16 once, because the tensor core takes
-// both operands of a product in one 16-bit type.
+// Sums, statistics, losses and picked logits are fp32. p - q is rounded to bf16 once, because the tensor core takes
+// both operands of a product in one 16-bit type; common factors (tau, 1 / count) are applied to the fp32 results
+// instead, where they cost no rounding and keep the large entries, targets near -1, at their finest steps. The
+// tensor core's running sum loses up to an ulp of it per 16 products, always towards zero: a cross-entropy's label,
+// whose logit enters alone, is therefore recomputed by fp32 fused multiply-adds while its row is gathered and
+// replaces the GEMM's value in lse, loss and G (error of the loss at H 4096: 4e-6 before).
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 
 #include <climits>
 #include <cmath>
+#include <tuple>
+#include <utility>
 
 #include "gemm_core.cuh"
 
@@ -41,7 +48,7 @@ namespace {
 
 constexpr int kNowhere = INT_MAX;  // a target outside this vocabulary (or padding of a target list)
 constexpr int kIgnored = -1;       // first target of a token that has none
-constexpr int kTile = 256;         // columns of a logits tile
+constexpr int kPad = 256;          // G's rows are whole logits tiles
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kCodeStep = 1024.f;  // fixed-point steps per power of two
 constexpr float kCodeMax = 65535.f;  // 64 powers of two below the maximum: stands for zero
@@ -60,29 +67,30 @@ struct HeadParams : GemmParams {
   const int* targets; // [tokens, n_targets], ascending
   int n_targets;
   float* picked;      // [rows, n_targets] base-2 logits of the targets
-  float2* part;       // [rows, n_tiles] (maximum, sum of 2^(x - maximum)) of each tile
+  float2* part;       // [rows, n_tiles] (maximum, sum of 2^(x - maximum)) of each BN / 2 columns
   int n_tiles;
   uint16_t* codes;    // [rows, ldg] distances (kCodes) or bf16 G (kGrad)
-  long ldg;           // a multiple of kTile
+  long ldg;           // a multiple of kPad
   const float* lse2;       // kGrad: [rows] base-2 log-sum-exp
   const float* row_scale;  // kGrad: [tokens] factor of G's rows
   float grad_scale;        // kGrad: and of all of G
 };
 
-// Epilogue of the logits GEMM. A thread owns one row of the tile; it reads the accumulator from TMEM twice, for the
-// maximum and for the sum, which costs less than keeping 256 values in registers or rescaling a running sum. The
-// sum's ex2 are the bound: 128 x 256 of them on 16 lanes a clock are 2048 clocks, hidden behind a main loop of
-// 8 H clocks a tile (CTA pair) from H = 256 on.
+// Epilogue of the logits GEMM. A thread owns half a row of the tile (128 columns in registers, read from TMEM
+// once). Eight warps share the tile, because its work, about ten instructions and one ex2 a logit, has to fit behind
+// the next tile's main loop of 8 H clocks: with four warps it took 14,000 clocks, more than a main loop up to
+// H = 1750 (measured at 2047 x 50257 x 768: 170 us).
 template <int MODE>
 struct HeadEpilogue {
   using Params = HeadParams;
+  static constexpr int kWarps = 8;
   const int* list = nullptr;  // this row's targets
   int pos = 0, next = kNowhere;
   float lse2 = 0.f, rs = 0.f;
 
   __device__ __forceinline__ HeadEpilogue(const Params&) {}
 
-  __device__ __forceinline__ void begin(const Params& p, long m0, int n0) {
+  __device__ __forceinline__ void begin(const Params& p, long m0, int c0) {
     const long m = m0 + (threadIdx.x & 31);
     next = kNowhere;
     int rows = p.M;
@@ -93,12 +101,12 @@ struct HeadEpilogue {
       lse2 = __ldg(p.lse2 + m);
       rs = __ldg(p.row_scale + token) * p.grad_scale;
     } else {
-      // The first target of the row at or after the tile's first column.
+      // The first target of the row at or after this thread's first column.
       list = p.targets + static_cast<long>(token) * p.n_targets;
       int lo = 0, hi = p.n_targets;
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (__ldg(list + mid) < n0) lo = mid + 1;
+        if (__ldg(list + mid) < c0) lo = mid + 1;
         else hi = mid;
       }
       pos = lo;
@@ -128,15 +136,17 @@ struct HeadEpilogue {
 
   template <int BN>
   __device__ __forceinline__ void tile(uint32_t t_row, float* stage_f, const Params& p, long m0, int n0, bool,
-                                       long m_end, int) {
-    static_assert(BN == kTile, "statistics are kept per 256 columns");
+                                       long m_end, int, int part) {
+    constexpr int COLS = BN / 2, GROUPS = COLS / 32;
     uint8_t* stage = reinterpret_cast<uint8_t*>(stage_f);
     const int lane = threadIdx.x & 31;
     const long m = m0 + lane;
-    const int ncol = min(BN, p.N - n0);  // columns of this tile that exist
+    n0 += part * COLS;
+    t_row += part * COLS;
+    const int ncol = p.N - n0;  // columns from here on that exist
     if constexpr (MODE == kGrad) {
 #pragma unroll 1
-      for (int g = 0; g < BN && g < ncol; g += 64) {
+      for (int g = 0; g < COLS && g < ncol; g += 64) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t r[32], w[16];
@@ -150,131 +160,206 @@ struct HeadEpilogue {
         flush(stage, p, m0, n0 + g, m_end);
       }
     } else {
-      float mx = -INFINITY;
-#pragma unroll 1
-      for (int g = 0; g < ncol; g += 32) {
-        uint32_t r[32];
-        tmem_ld32(t_row + g, r);
-        if (g + 32 <= ncol) {
+      uint32_t r[GROUPS][32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(r[j]));
-        } else {
+      for (int g = 0; g < GROUPS; ++g) tmem_ld32(t_row + g * 32, r[g]);
+      if (ncol < COLS) {  // the vocabulary ends in here
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            if (g + j < ncol) mx = fmaxf(mx, __uint_as_float(r[j]));
-        }
+            if (g * 32 + j >= ncol) r[g][j] = 0xff800000u;  // -inf
       }
-      const float m2 = mx == -INFINITY ? 0.f : mx * p.scale2;  // -inf logits count 0, not NaN
+      float mx = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(r[g][j]));
+      const float ref = mx == -INFINITY ? 0.f : mx;  // columns all at -inf sum to 0, not NaN
+      const float neg_step = -p.scale2 * kCodeStep;
       float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-      for (int g = 0; g < ncol; g += 64) {
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          const int c0 = g + half * 32;
-          uint32_t r[32];
-          tmem_ld32(t_row + c0, r);  // columns past ncol hold zeros: read, not counted
-          const bool whole = c0 + 32 <= ncol;
-          uint32_t w[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float d = fmaf(__uint_as_float(r[j]), p.scale2, -m2);  // <= 0 up to rounding
-            const float e = ex2(d);
-            if (whole || c0 + j < ncol) s[j & 3] += e;
-            if constexpr (MODE == kCodes) {
-              // Adding 2^23 leaves the rounded distance in the low mantissa bits.
-              const float t = fminf(fmaxf(fmaf(d, -kCodeStep, 8388608.f), 8388608.f), 8388608.f + kCodeMax);
-              if (j & 1) w[j >> 1] = __byte_perm(w[j >> 1], __float_as_uint(t), 0x5410);
-              else w[j >> 1] = __float_as_uint(t);
-            }
-          }
-          // Targets are rare (K of V columns): a round of the loop serves one of every row of the warp.
-          while (__any_sync(0xffffffffu, next < n0 + c0 + 32)) {
-            const int rel = next - n0 - c0;
-            float v = 0.f;
+      for (int g = 0; g < GROUPS; ++g) {
+        uint32_t w[16];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v = rel == j ? __uint_as_float(r[j]) : v;
-            if (next < n0 + c0 + 32) {
-              p.picked[m * p.n_targets + pos] = v * p.scale2;
-              ++pos;
-              next = pos < p.n_targets ? __ldg(list + pos) : kNowhere;
-            }
+        for (int j = 0; j < 32; ++j) {
+          const float d = __uint_as_float(r[g][j]) - ref;  // <= 0
+          s[j & 3] += ex2(d * p.scale2);
+          if constexpr (MODE == kCodes) {
+            // Adding 2^23 leaves the rounded distance in the low mantissa bits.
+            const float t = fminf(fmaf(d, neg_step, 8388608.f), 8388608.f + kCodeMax);
+            if (j & 1) w[j >> 1] = __byte_perm(w[j >> 1], __float_as_uint(t), 0x5410);
+            else w[j >> 1] = __float_as_uint(t);
           }
-          if constexpr (MODE == kCodes) put(stage, w, half);
         }
-        if constexpr (MODE == kCodes) flush(stage, p, m0, n0 + g, m_end);
+        // Targets are rare (K of V columns): a round of the loop serves one of every row of the warp.
+        const int c0 = n0 + g * 32;
+        while (__any_sync(0xffffffffu, next < c0 + 32)) {
+          const int rel = next - c0;
+          float v = 0.f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v = rel == j ? __uint_as_float(r[g][j]) : v;
+          if (next < c0 + 32) {
+            p.picked[m * p.n_targets + pos] = v * p.scale2;
+            ++pos;
+            next = pos < p.n_targets ? __ldg(list + pos) : kNowhere;
+          }
+        }
+        if constexpr (MODE == kCodes) {
+          put(stage, w, g & 1);
+          if (g & 1) flush(stage, p, m0, n0 + (g - 1) * 32, m_end);
+        }
       }
       if (m < m_end)
-        p.part[m * p.n_tiles + n0 / BN] = make_float2(mx == -INFINITY ? mx : m2, (s[0] + s[1]) + (s[2] + s[3]));
+        p.part[m * p.n_tiles + n0 / COLS] = make_float2(mx * p.scale2, (s[0] + s[1]) + (s[2] + s[3]));
     }
   }
 };
 
 // ------------------------------------------------------------------ token rows
-// Targets of a cross-entropy: the label's column in this shard, kNowhere outside it, kIgnored for ignore_index.
-// With labels == nullptr the targets are already there. Compacts the tokens that have a target: map[r] = token of
-// compact row r, place[t] = compact row or -1, *count their number; the losses of the others are set to 0.
-// One CTA: a serial scan over T tokens, 8192 a round (3.4 us at 16384 tokens).
-__global__ void __launch_bounds__(1024)
-    head_rows_kernel(const int64_t* __restrict__ labels, int64_t vstart, int64_t V, int64_t ignore_index,
-                     int* __restrict__ targets, int n_targets, int T, int* __restrict__ map, int* __restrict__ place,
-                     int* __restrict__ count, float* __restrict__ loss) {
-  constexpr int kItems = 8;
-  __shared__ int sums[kItems * 32];
-  __shared__ int total;
+// What later kernels and the backward pass need of a call, in one buffer.
+struct Header {
+  int count;     // live tokens
+  int ticket;    // row CTAs that are done
+  float inv;     // 1 / count for a mean, else 1
+  int pad[13];
+};
+
+struct StateView {
+  Header* head;
+  int* targets;     // [T, K] ascending, kNowhere past the end; kIgnored first where the token has none
+  int* map;         // [T] compact row -> token
+  int* place;       // [T] token -> compact row, -1
+  float* loss;      // [T]
+  float* lse2;      // [T] compact
+  float* picked;    // [T, K] compact
+  float* exact;     // [T] compact: the label's fp32 logit (cross-entropy)
+  int* live;        // [T] (distillation)
+  float* q;         // [T, K] (distillation)
+  float* constant;  // [T] sum q log q (distillation)
+};
+
+struct GatherParams {
+  const bf16* h;
+  long ldh;
+  const bf16* w;  // cross-entropy: for the labels' logits
+  long ldw;
+  int H, T;
+  const int64_t* labels;  // nullptr: distillation
+  int64_t vstart, V, ignore_index;
+  int mean;
+  float scale2;
+  StateView st;
+  bf16* x;    // [round_up(T, 64), H]
+  bf16* dh;   // optional: rows of tokens without a target are zeroed
+  int tokens; // per CTA
+};
+
+constexpr int kGatherThreads = 256;
+
+__device__ __forceinline__ void zero_row(bf16* dst, int H) {
+  for (int i = threadIdx.x & 31; i < H / 8; i += 32) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// Takes the tokens that have a target out into consecutive rows, in order. Each CTA counts the live tokens before
+// its own by reading the labels itself (T / tokens CTAs x T labels out of L2: 2 us at 16384 tokens), which saves a
+// scan launch and a pass; a warp then copies a row and, for a cross-entropy, forms the label's logit from it. The
+// rows up to the next multiple of 64 are zeroed, because the weight gradient's K blocks reach that far. With KNOWN,
+// the places are there already and only the rows are copied.
+template <bool KNOWN>
+__global__ void __launch_bounds__(kGatherThreads) head_gather_kernel(GatherParams p) {
+  __shared__ int red[2][kGatherThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int base = 0;
-  for (int t0 = 0; t0 < T; t0 += kItems * 1024) {
-    int before[kItems];
-    bool live[kItems];
-#pragma unroll
-    for (int j = 0; j < kItems; ++j) {
-      const int t = t0 + j * 1024 + static_cast<int>(threadIdx.x);
-      live[j] = false;
-      if (t < T) {
-        if (labels != nullptr) {
-          const int64_t lab = labels[t], rel = lab - vstart;
-          live[j] = lab != ignore_index;
-          targets[t] = !live[j] ? kIgnored : (rel >= 0 && rel < V ? static_cast<int>(rel) : kNowhere);
-        } else {
-          live[j] = targets[static_cast<long>(t) * n_targets] != kIgnored;
-        }
-      }
-      const unsigned b = __ballot_sync(0xffffffffu, live[j]);
-      before[j] = __popc(b & ((1u << lane) - 1u));
-      if (lane == 0) sums[j * 32 + warp] = __popc(b);
+  const int t0 = blockIdx.x * p.tokens, t1 = min(p.T, t0 + p.tokens);
+  auto live = [&](int t) { return p.labels != nullptr ? p.labels[t] != p.ignore_index : p.st.live[t] != 0; };
+  int before = 0, count = 0;
+  if constexpr (KNOWN) {
+    count = p.st.head->count;
+  } else {
+#pragma unroll 4
+    for (int t = threadIdx.x; t < p.T; t += kGatherThreads) {
+      const int l = live(t) ? 1 : 0;
+      count += l;
+      before += t < t0 ? l : 0;
+    }
+    count = __reduce_add_sync(0xffffffffu, count);
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0) {
+      red[0][warp] = count;
+      red[1][warp] = before;
     }
     __syncthreads();
-    if (warp == 0) {  // exclusive scan of the 256 warp counts, 8 to a lane
-      int v[kItems], run = 0;
+    count = before = 0;
 #pragma unroll
-      for (int i = 0; i < kItems; ++i) {
-        v[i] = run;
-        run += sums[lane * kItems + i];
-      }
-      int inc = run;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int n = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += n;
-      }
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) sums[lane * kItems + i] = v[i] + inc - run;
-      if (lane == 31) total = inc;
+    for (int i = 0; i < kGatherThreads / 32; ++i) {
+      count += red[0][i];
+      before += red[1][i];
     }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kItems; ++j) {
-      const int t = t0 + j * 1024 + static_cast<int>(threadIdx.x);
-      if (t >= T) continue;
-      const int r = base + sums[j * 32 + warp] + before[j];
-      place[t] = live[j] ? r : -1;
-      if (live[j]) map[r] = t;
-      else loss[t] = 0.f;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      p.st.head->count = count;
+      p.st.head->ticket = 0;
+      p.st.head->inv = p.mean ? 1.f / static_cast<float>(max(count, 1)) : 1.f;
     }
-    base += total;
-    __syncthreads();
   }
-  if (threadIdx.x == 0) *count = base;
+  const int vecs = p.H / 8;
+  // Every warp walks all of the CTA's tokens to know their places (32 at a time) and copies its share.
+  for (int b = t0; b < t1; b += 32) {
+    const int mine = b + lane;
+    int place = -1;
+    if constexpr (KNOWN) {
+      if (mine < t1) place = p.st.place[mine];
+    } else {
+      const bool l = mine < t1 && live(mine);
+      const unsigned mask = __ballot_sync(0xffffffffu, l);
+      if (l) place = before + __popc(mask & ((1u << lane) - 1u));
+      before += __popc(mask);
+      if (warp == 0 && mine < t1) {
+        p.st.place[mine] = place;
+        if (l) p.st.map[place] = mine;
+        else p.st.loss[mine] = 0.f;
+      }
+    }
+    for (int i = warp; i < 32 && b + i < t1; i += kGatherThreads / 32) {
+      const int t = b + i, row = __shfl_sync(0xffffffffu, place, i);
+      int target = kIgnored;
+      if (!KNOWN && p.labels != nullptr) {
+        const int64_t rel = p.labels[t] - p.vstart;
+        if (row >= 0) target = rel >= 0 && rel < p.V ? static_cast<int>(rel) : kNowhere;
+        if (lane == 0) p.st.targets[t] = target;
+      }
+      if (row < 0) {
+        if (!KNOWN && p.dh != nullptr) zero_row(p.dh + static_cast<long>(t) * p.H, p.H);
+        continue;
+      }
+      const uint4* src = reinterpret_cast<const uint4*>(p.h + t * p.ldh);
+      uint4* dst = reinterpret_cast<uint4*>(p.x + static_cast<long>(row) * p.H);
+      if (target >= 0 && target != kNowhere) {
+        const uint4* wr = reinterpret_cast<const uint4*>(p.w + target * p.ldw);
+        float dot[2] = {0.f, 0.f};
+#pragma unroll 4
+        for (int k = lane; k < vecs; k += 32) {
+          const uint4 a = __ldg(src + k), c = __ldg(wr + k);
+          dst[k] = a;
+          dot[0] = fmaf(bf16_lo(a.x), bf16_lo(c.x), dot[0]);
+          dot[1] = fmaf(bf16_hi(a.x), bf16_hi(c.x), dot[1]);
+          dot[0] = fmaf(bf16_lo(a.y), bf16_lo(c.y), dot[0]);
+          dot[1] = fmaf(bf16_hi(a.y), bf16_hi(c.y), dot[1]);
+          dot[0] = fmaf(bf16_lo(a.z), bf16_lo(c.z), dot[0]);
+          dot[1] = fmaf(bf16_hi(a.z), bf16_hi(c.z), dot[1]);
+          dot[0] = fmaf(bf16_lo(a.w), bf16_lo(c.w), dot[0]);
+          dot[1] = fmaf(bf16_hi(a.w), bf16_hi(c.w), dot[1]);
+        }
+        const float sum = warp_sum(dot[0] + dot[1]);
+        if (lane == 0) p.st.exact[row] = sum * p.scale2;
+      } else {
+#pragma unroll 4
+        for (int k = lane; k < vecs; k += 32) dst[k] = __ldg(src + k);
+      }
+    }
+  }
+  for (int r = count + blockIdx.x * (kGatherThreads / 32) + warp; r < max(64, (count + 63) & ~63);
+       r += gridDim.x * (kGatherThreads / 32))
+    if (r < ((p.T + 63) & ~63)) zero_row(p.x + static_cast<long>(r) * p.H, p.H);
 }
 
 // Targets of a distillation: one CTA sorts a token's K (index, teacher value) pairs by index and turns the values
@@ -283,7 +368,7 @@ __global__ void __launch_bounds__(1024)
 template <typename T, typename I>
 __global__ void head_teacher_kernel(const T* __restrict__ values, long ldv, const I* __restrict__ indices, long ldi,
                                     int K, int P, float inv_tau, int64_t V, int* __restrict__ targets,
-                                    float* __restrict__ q, float* __restrict__ constant) {
+                                    int* __restrict__ live, float* __restrict__ q, float* __restrict__ constant) {
   extern __shared__ int teacher_smem[];
   int* key = teacher_smem;
   float* val = reinterpret_cast<float*>(teacher_smem + P);
@@ -347,51 +432,44 @@ __global__ void head_teacher_kernel(const T* __restrict__ values, long ldv, cons
     if (there) ent += p * (val[k] - logz);
   }
   ent = block(ent, false);
-  if (threadIdx.x == 0) constant[t] = ent;
-}
-
-// Compact copy of the live tokens' hidden states; the rows up to the next multiple of 64 are zeroed, because the
-// weight gradient's K blocks reach that far.
-__global__ void head_gather_kernel(const bf16* __restrict__ h, long ldh, int H, int T, const int* __restrict__ map,
-                                   const int* __restrict__ count, bf16* __restrict__ x) {
-  const int row = blockIdx.x, n = *count;
-  if (row >= ((n + 63) & ~63) && row >= 64) return;
-  const int vecs = H / 8;
-  uint4* dst = reinterpret_cast<uint4*>(x + static_cast<long>(row) * H);
-  if (row >= n) {
-    for (int i = threadIdx.x; i < vecs; i += blockDim.x) dst[i] = make_uint4(0, 0, 0, 0);
-    return;
+  if (threadIdx.x == 0) {
+    constant[t] = ent;
+    live[t] = none ? 0 : 1;
   }
-  const uint4* src = reinterpret_cast<const uint4*>(h + static_cast<long>(map[row]) * ldh);
-  for (int i = threadIdx.x; i < vecs; i += blockDim.x) dst[i] = __ldg(src + i);
 }
 
 // ------------------------------------------------------------------ rows of a chunk
 struct RowParams {
-  const int* rows;  // device count of live tokens
+  const Header* head;
   int rows_base;    // first compact row of the chunk
-  const int* map;
+  const int* map;   // from the chunk's first row on, as the other arrays over compact rows
   const int* targets;
   const float* q;         // [tokens, K] target weights; nullptr: 1 (K = 1)
   const float* constant;  // [tokens] added to the loss; nullptr: 0
   int K;
-  const float* picked;  // [rows, K]
-  const float2* part;   // [rows, n_tiles]
+  float* picked;       // [rows, K]
+  const float* exact;  // [rows] fp32 logit of the one target, or nullptr
+  const float2* part;  // [rows, n_tiles]
   int n_tiles;
+  int tile_shift;  // log2 of a statistics tile's 8-column vectors
   uint16_t* codes;
   long ldg;
   int V;
   float* loss;  // [tokens]
-  float* lse2;  // [rows], optional
+  float* lse2;  // [rows]
   float loss_scale;
-  float grad_scale;  // of G, further divided by the number of live tokens when `mean`
-  int mean;
+  float grad_scale;  // head_fix_kernel
+  // The last of `tickets` CTAs (over all chunks) to finish adds up the T losses; tickets 0: nobody does.
+  int* ticket;
+  int tickets;
+  int T;
+  float* out;
 };
 
 constexpr int kRowThreads = 512;
 
-__device__ __forceinline__ float row_join(float2& a, float2* red, int nwarp) {
-  // Joins (max, sum) pairs over the block; every thread returns log2 of the whole sum.
+// Joins (maximum, sum) pairs over the block; every thread returns log2 of the whole sum.
+__device__ __forceinline__ float row_join(float2 a, float2* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto merge = [](float2 x, float2 y) {
     const float m = fmaxf(x.x, y.x);
@@ -404,90 +482,112 @@ __device__ __forceinline__ float row_join(float2& a, float2* red, int nwarp) {
   if (lane == 0) red[warp] = a;
   __syncthreads();
   a = red[0];
-  for (int w = 1; w < nwarp; ++w) a = merge(a, red[w]);
+#pragma unroll
+  for (int w = 1; w < kRowThreads / 32; ++w) a = merge(a, red[w]);
   return a.x + log2f(a.y);
 }
 
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = red[0];
+#pragma unroll
+  for (int w = 1; w < kRowThreads / 32; ++w) s += red[w];
+  return s;
+}
+
+// 2^(base - code / 1024). The code becomes a float by putting it under the exponent of 2^23: the conversion unit
+// shares its rate with ex2, which would bound the kernel. The last code stands for zero; NaN statistics stay NaN.
 __device__ __forceinline__ float code_prob(uint32_t code, float base) {
-  // The last code stands for zero; NaN statistics still give NaN.
-  const float d = code == 65535u ? -INFINITY : static_cast<float>(code) * (-1.f / kCodeStep);
-  return ex2(base + d);
+  const float c = __uint_as_float(0x4b000000u | code) - 8388608.f;
+  return ex2(fmaf(c, -1.f / kCodeStep, code == 65535u ? base - INFINITY : base));
 }
 
 // One CTA per compact row: statistics -> lse, loss; with WRITE also distances -> G in place. G's pass reads and
 // writes 2 bytes an entry once, so the kernel is bound by memory.
 template <bool WRITE>
 __global__ void __launch_bounds__(kRowThreads) head_row_kernel(RowParams p) {
-  extern __shared__ float row_smem[];  // WRITE: the tiles' maxima, relative to lse
+  extern __shared__ float row_smem[];  // WRITE: the tiles' maxima
   __shared__ float2 red2[kRowThreads / 32];
   __shared__ float red[kRowThreads / 32];
-  const int live = min(max(*p.rows - p.rows_base, 0), static_cast<int>(gridDim.x));
-  const int row = blockIdx.x, total = *p.rows;
-  if (row >= live) {
-    if (WRITE && row < max(64, (live + 63) & ~63)) {
+  __shared__ int last;
+  const int live = min(max(p.head->count - p.rows_base, 0), static_cast<int>(gridDim.x));
+  const int row = blockIdx.x;
+  if (row < live) {
+    const int token = p.map[row];
+    const float2* part = p.part + static_cast<long>(row) * p.n_tiles;
+    float2 a = make_float2(-INFINITY, 0.f);
+    for (int i = threadIdx.x; i < p.n_tiles; i += kRowThreads) {
+      const float2 b = part[i];
+      if (WRITE) row_smem[i] = b.x;
+      const float m = fmaxf(a.x, b.x);
+      a = make_float2(m, (a.x == m ? a.y : a.y * ex2(a.x - m)) + (b.x == m ? b.y : b.y * ex2(b.x - m)));
+    }
+    float lse2 = row_join(a, red2);
+    const int* targets = p.targets + static_cast<long>(token) * p.K;
+    const float* q = p.q ? p.q + static_cast<long>(token) * p.K : nullptr;
+    float* picked = p.picked + static_cast<long>(row) * p.K;
+    float only = 0.f;  // the one target's logit; 0 for a label of another shard, whose rank has it
+    if (p.exact != nullptr && targets[0] != kNowhere) {
+      // The label's logit in fp32 takes the place of the GEMM's in the sum.
+      only = p.exact[row];
+      lse2 += log1pf(ex2(only - lse2) - ex2(picked[0] - lse2)) * (1.f / kLn2);
+    }
+    if constexpr (WRITE) {
       uint4* g = reinterpret_cast<uint4*>(p.codes + row * p.ldg);
-      for (long i = threadIdx.x; i < p.ldg / 8; i += kRowThreads) g[i] = make_uint4(0, 0, 0, 0);
-    }
-    return;
-  }
-  const int token = p.map[row];
-  const float2* part = p.part + static_cast<long>(row) * p.n_tiles;
-  float2 a = make_float2(-INFINITY, 0.f);
-  for (int i = threadIdx.x; i < p.n_tiles; i += kRowThreads) {
-    const float2 b = part[i];
-    if (WRITE) row_smem[i] = b.x;
-    const float m = fmaxf(a.x, b.x);
-    a = make_float2(m, (a.x == m ? a.y : a.y * ex2(a.x - m)) + (b.x == m ? b.y : b.y * ex2(b.x - m)));
-  }
-  const float lse2 = row_join(a, red2, kRowThreads / 32);
-  const int* targets = p.targets + static_cast<long>(token) * p.K;
-  const float* q = p.q ? p.q + static_cast<long>(token) * p.K : nullptr;
-  const float* picked = p.picked + static_cast<long>(row) * p.K;
-  float scale = p.grad_scale;
-  if (p.mean) scale /= static_cast<float>(max(total, 1));
-  if constexpr (WRITE) {
-    __syncthreads();
-    uint4* g = reinterpret_cast<uint4*>(p.codes + row * p.ldg);
-    const int vecs = (p.V + 7) / 8;
+      const int vecs = (p.V + 7) / 8;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < vecs; i += kRowThreads) {
-      const uint4 c = g[i];
-      const float base = row_smem[i >> 5] - lse2;
-      const uint32_t in[4] = {c.x, c.y, c.z, c.w};
-      uint32_t out[4];
+      for (int i = threadIdx.x; i < vecs; i += kRowThreads) {
+        const uint4 c = g[i];
+        const float base = row_smem[i >> p.tile_shift] - lse2;
+        const uint32_t in[4] = {c.x, c.y, c.z, c.w};
+        uint32_t out[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        out[j] = pack_bf16x2(code_prob(in[j] & 0xffffu, base) * scale, code_prob(in[j] >> 16, base) * scale);
-      g[i] = make_uint4(out[0], out[1], out[2], out[3]);
+        for (int j = 0; j < 4; ++j) out[j] = pack_bf16x2(code_prob(in[j] & 0xffffu, base), code_prob(in[j] >> 16, base));
+        g[i] = make_uint4(out[0], out[1], out[2], out[3]);
+      }
     }
-    __syncthreads();
-  }
-  float loss = 0.f;
-  for (int k = threadIdx.x; k < p.K; k += kRowThreads) {
-    const int j = targets[k];
-    const float x2 = j == kNowhere ? 0.f : picked[k];  // a label of another shard: that rank has its logit
-    const float qk = q ? q[k] : 1.f;
-    if (j != kNowhere || q == nullptr) loss += qk * (lse2 - x2);
-    if (WRITE && j != kNowhere && (k == 0 || targets[k - 1] != j)) {
-      float sum = qk;
-      for (int i = k + 1; i < p.K && targets[i] == j; ++i) sum += q[i];
-      reinterpret_cast<bf16*>(p.codes + row * p.ldg)[j] = __float2bfloat16((ex2(x2 - lse2) - sum) * scale);
+    __syncthreads();  // all have read `picked`, and G's pass is done
+    float loss = 0.f;
+    for (int k = threadIdx.x; k < p.K; k += kRowThreads) {
+      const int j = targets[k];
+      const float x2 = p.exact != nullptr ? only : (j == kNowhere ? 0.f : picked[k]);
+      const float qk = q ? q[k] : 1.f;
+      if (j != kNowhere || q == nullptr) loss += qk * (lse2 - x2);
+      if (p.exact != nullptr) picked[0] = only;
+      if (WRITE && j != kNowhere && (k == 0 || targets[k - 1] != j)) {
+        float sum = qk;
+        for (int i = k + 1; i < p.K && targets[i] == j; ++i) sum += q[i];
+        reinterpret_cast<bf16*>(p.codes + row * p.ldg)[j] = __float2bfloat16(ex2(x2 - lse2) - sum);
+      }
     }
+    loss = row_sum(loss, red);
+    if (threadIdx.x == 0) {
+      p.loss[token] = (loss * kLn2 + (p.constant ? p.constant[token] : 0.f)) * p.loss_scale;
+      p.lse2[row] = lse2;
+    }
+  } else if (WRITE && row < max(64, (live + 63) & ~63)) {
+    uint4* g = reinterpret_cast<uint4*>(p.codes + row * p.ldg);
+    for (long i = threadIdx.x; i < p.ldg / 8; i += kRowThreads) g[i] = make_uint4(0, 0, 0, 0);
   }
-  loss = warp_sum(loss);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = loss;
-  __syncthreads();
+  if (p.tickets == 0) return;
   if (threadIdx.x == 0) {
-    float s = red[0];
-    for (int w = 1; w < kRowThreads / 32; ++w) s += red[w];
-    p.loss[token] = (s * kLn2 + (p.constant ? p.constant[token] : 0.f)) * p.loss_scale;
-    if (p.lse2) p.lse2[row] = lse2;
+    __threadfence();
+    last = atomicAdd(p.ticket, 1) == p.tickets - 1 ? 1 : 0;
+    __threadfence();
   }
+  __syncthreads();
+  if (last == 0) return;
+  float s = 0.f;
+  for (int t = threadIdx.x; t < p.T; t += kRowThreads) s += __ldcg(p.loss + t);
+  s = row_sum(s, red);
+  if (threadIdx.x == 0) *p.out = s * p.head->inv;
 }
 
 // Targets' entries of a G that the kGrad epilogue wrote, and the zero rows up to the next multiple of 64.
 __global__ void head_fix_kernel(RowParams p, const float* __restrict__ row_scale) {
-  const int live = min(max(*p.rows - p.rows_base, 0), static_cast<int>(gridDim.x));
+  const int live = min(max(p.head->count - p.rows_base, 0), static_cast<int>(gridDim.x));
   const int row = blockIdx.x;
   if (row >= live) {
     if (row < max(64, (live + 63) & ~63)) {
@@ -509,10 +609,11 @@ __global__ void head_fix_kernel(RowParams p, const float* __restrict__ row_scale
   }
 }
 
-// Adds dH's K slices in order and puts the compact rows back to their tokens; tokens without a target get zeros.
-__global__ void head_dh_kernel(const float* __restrict__ part, int slices, long slice_stride, int H,
-                               const int* __restrict__ place, int row_base, int row_end, int zero_others,
-                               bf16* __restrict__ dh) {
+// Adds dH's K slices in order, scales the sum by alpha (* *alpha_dev) and puts the compact rows back to their
+// tokens. The rows of tokens without a target were zeroed by the gather, or here with zero_others.
+__global__ void head_dh_kernel(const float* __restrict__ part, int slices, long slice_stride, int H, float alpha,
+                               const float* __restrict__ alpha_dev, const int* __restrict__ place, int row_base,
+                               int row_end, int zero_others, bf16* __restrict__ dh) {
   const long t = blockIdx.x;
   const int r = place[t];
   uint2* out = reinterpret_cast<uint2*>(dh + t * H);
@@ -522,9 +623,11 @@ __global__ void head_dh_kernel(const float* __restrict__ part, int slices, long 
     return;
   }
   if (r < row_base || r >= row_end) return;
+  if (alpha_dev != nullptr) alpha *= *alpha_dev;
   const float* src = part + static_cast<long>(r - row_base) * H;
   for (int i = threadIdx.x; i < H / 4; i += blockDim.x) {
     float4 a = *reinterpret_cast<const float4*>(src + i * 4);
+#pragma unroll 4
     for (int s = 1; s < slices; ++s) {
       const float4 b = *reinterpret_cast<const float4*>(src + s * slice_stride + i * 4);
       a.x += b.x;
@@ -532,97 +635,69 @@ __global__ void head_dh_kernel(const float* __restrict__ part, int slices, long 
       a.z += b.z;
       a.w += b.w;
     }
-    out[i] = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+    out[i] = make_uint2(pack_bf16x2(a.x * alpha, a.y * alpha), pack_bf16x2(a.z * alpha, a.w * alpha));
   }
 }
 
-// out = sum of the tokens' losses, in a fixed order, divided by the number of live tokens when `mean`.
-__global__ void __launch_bounds__(1024)
-    head_loss_kernel(const float* __restrict__ loss, int T, const int* __restrict__ count, int mean,
-                     float* __restrict__ out) {
-  __shared__ float red[32];
-  float s = 0.f;
-  for (int t = threadIdx.x; t < T; t += 1024) s += loss[t];
-  s = warp_sum(s);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    s = warp_sum(red[threadIdx.x]);
-    if (threadIdx.x == 0) *out = mean ? s / static_cast<float>(max(*count, 1)) : s;
-  }
-}
-
-// x *= *factor, in place; nothing is read or written when the factor is 1 (a loss that is itself the root).
-template <typename T>
-__global__ void head_scale_kernel(T* __restrict__ x, int64_t n, const float* __restrict__ factor) {
+// Two bf16 buffers (either may be empty) times *factor, in place; nothing is read or written when the factor is 1
+// (a loss that is itself the root of the backward pass).
+__global__ void __launch_bounds__(256)
+    head_scale_kernel(bf16* __restrict__ a, int64_t na, bf16* __restrict__ b, int64_t nb,
+                      const float* __restrict__ factor) {
   const float f = *factor;
   if (f == 1.f) return;
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 8; i < n;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x * 8) {
-    if (i + 8 <= n) {
-      if constexpr (sizeof(T) == 2) {
-        uint4 v = *reinterpret_cast<uint4*>(x + i);
-        uint32_t* w = &v.x;
+  const int64_t va = na / 8, total = va + nb / 8;  // rows are whole vectors
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    uint4* at = reinterpret_cast<uint4*>(i < va ? a : b) + (i < va ? i : i - va);
+    uint4 v = *at;
+    uint32_t* w = &v.x;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(bf16_lo(w[j]) * f, bf16_hi(w[j]) * f);
-        *reinterpret_cast<uint4*>(x + i) = v;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float4 v = *reinterpret_cast<float4*>(x + i + 4 * j);
-          v.x *= f;
-          v.y *= f;
-          v.z *= f;
-          v.w *= f;
-          *reinterpret_cast<float4*>(x + i + 4 * j) = v;
-        }
-      }
-    } else {
-      for (int64_t j = i; j < n; ++j) x[j] = static_cast<T>(static_cast<float>(x[j]) * f);
-    }
+    for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(bf16_lo(w[j]) * f, bf16_hi(w[j]) * f);
+    *at = v;
   }
 }
 
 // dst = or += factor * src, src fp32.
 template <typename T, bool ADD>
-__global__ void head_scaled_copy_kernel(const float* __restrict__ src, int64_t n, const float* __restrict__ factor,
-                                        T* __restrict__ dst) {
+__global__ void __launch_bounds__(256)
+    head_scaled_copy_kernel(const float* __restrict__ src, int64_t n, const float* __restrict__ factor,
+                            T* __restrict__ dst) {
   const float f = factor ? *factor : 1.f;
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 4; i < n;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x * 4) {
-    if (i + 4 <= n) {
-      const float4 v = *reinterpret_cast<const float4*>(src + i);
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint2*>(dst + i) = make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
-      } else {
-        float4 o = ADD ? *reinterpret_cast<const float4*>(dst + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-        *reinterpret_cast<float4*>(dst + i) = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z),
-                                                          fmaf(v.w, f, o.w));
-      }
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4; i < n;
+       i += static_cast<int64_t>(gridDim.x) * 256 * 4) {
+    const float4 v = *reinterpret_cast<const float4*>(src + i);
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint2*>(dst + i) = make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
     } else {
-      for (int64_t j = i; j < n; ++j)
-        dst[j] = static_cast<T>(src[j] * f + (ADD ? static_cast<float>(dst[j]) : 0.f));
+      const float4 o = ADD ? *reinterpret_cast<const float4*>(dst + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<float4*>(dst + i) = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z),
+                                                        fmaf(v.w, f, o.w));
     }
   }
 }
 
-int stream_blocks(int64_t n, int per_block) {
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((n + per_block - 1) / per_block, 148 * 8)));
+unsigned stream_blocks(int64_t n, int per_block) {
+  return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((n + per_block - 1) / per_block, 148 * 8)));
 }
 
 // ------------------------------------------------------------------ host side
 int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
-// A rows-by-H view that a tensor map takes as it is.
-void check_operand(const at::Tensor& t, const char* what) {
-  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && t.scalar_type() == at::kBFloat16, what, ": 2-D bf16 CUDA tensor");
-  TORCH_CHECK(t.stride(1) == 1 && t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0,
-              what, ": unit inner stride, rows on 16-byte boundaries");
+// The 2-D rows of a tensor as the tensor maps take them: unit inner stride, every row on a 16-byte boundary.
+at::Tensor rows_operand(const at::Tensor& t) {
+  auto r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  const bool ok = r.stride(1) == 1 && r.stride(0) % 8 == 0 && (r.size(0) <= 1 || r.stride(0) >= r.size(1)) &&
+                  (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15) == 0;
+  return ok ? r : r.clone(at::MemoryFormat::Contiguous);
 }
 
-// The logits GEMM over a chunk. Few tokens run on single-CTA tiles of 128 rows; from 256 rows on the CTA pair
-// halves the traffic of each operand (as for the plain GEMM, whose pair rule needs K >= 2048; here the pair's
-// longer prologue hides behind the wide N loop, so rows alone decide).
+// The logits GEMM over a chunk. Up to 128 rows the weight is streamed once and bandwidth decides: 128-column tiles
+// fill the last wave of CTAs better (17 rows, V 128256: 6.8 waves against 3.4 of 256 columns). From 256 rows on the CTA
+// pair halves each operand's traffic; the plain GEMM's rule asks for K >= 2048 as well, here the pair's longer
+// prologue is spread over the wide N loop.
+int logits_tile(int64_t rows) { return rows <= 128 ? 128 : 256; }
+
 template <int MODE>
 void launch_logits(const at::Tensor& x, const at::Tensor& w, HeadParams p, cudaStream_t stream) {
   TmaSlots& slots = tls_tma_slots();
@@ -630,26 +705,31 @@ void launch_logits(const at::Tensor& x, const at::Tensor& w, HeadParams p, cudaS
   if (p.M >= 256) {
     operand_map(&slots.m[1], w, false, 128);
     launch_gemm_pair<false, false, HeadEpilogue<MODE>>(&slots.m[0], &slots.m[1], p, stream);
-  } else {
+  } else if (logits_tile(p.M) == 256) {
     operand_map(&slots.m[1], w, false, 256);
     launch_gemm<256, false, false, 0, HeadEpilogue<MODE>>(&slots.m[0], &slots.m[1], p, stream);
+  } else {
+    operand_map(&slots.m[1], w, false, 128);
+    launch_gemm<128, false, false, 0, HeadEpilogue<MODE>>(&slots.m[0], &slots.m[1], p, stream);
   }
 }
 
-// Slices of the vocabulary for dH: the 256 x 256 pair tiles (128 x 256 below 256 rows) of [rows, H] rarely fill the
-// SMs a whole number of times, and few tokens leave most of them idle. Modelled time: waves x (K blocks x 0.30 us +
-// 4 us a unit), plus writing and reading back the fp32 partials.
+// Slices of the vocabulary for dH. Its 256 x 256 pair tiles (128 x 256 below 256 rows) rarely fill the SMs a whole
+// number of times, by how much only the device knows (the live tokens), and few tokens leave most SMs idle. Modelled
+// time: (waves + half a wave that the last one wastes on average) x (K blocks x 0.30 us + 4 us a unit), plus writing
+// and reading back the fp32 partials.
 int pick_slices(int64_t rows, int64_t H, int64_t V, int nsm) {
   const bool pair = rows >= 256;
   const int64_t units = (pair ? (rows + 255) / 256 : (rows + 127) / 128) * ((H + 255) / 256);
-  const int64_t slots = pair ? nsm / 2 : nsm, kb = (V + 63) / 64;
+  const double slots = pair ? nsm / 2 : nsm;
+  const int64_t kb = (V + 63) / 64;
   double best = 1e30;
   int pick = 1;
   for (int64_t s = 1; s <= 148; ++s) {
     const int64_t per = (kb + s - 1) / s;
     if (s > 1 && (per < 4 || (kb + per - 1) / per != s)) continue;  // no empty slice
     if (s > 1 && pair && per < 32) break;                           // 2048 of K, where pairs pay
-    const double waves = static_cast<double>((units * s + slots - 1) / slots);
+    const double waves = std::max(1.0, units * s / slots + 0.5);
     const double us = waves * (per * 0.30 + 4.0) + s * rows * H * 8.0 / 6.0e6;
     if (us < best * 0.99) {
       best = us;
@@ -664,75 +744,120 @@ struct Head {
   int64_t T, H, V;
   int dev;
   cudaStream_t stream;
-  at::TensorOptions f32, i32;
 
-  Head(const at::Tensor& h_, const at::Tensor& w_) : h(h_), w(w_) {
-    check_operand(h, "linear head hidden");
-    check_operand(w, "linear head weight");
+  Head(const at::Tensor& hidden, const at::Tensor& weight) : h(rows_operand(hidden)), w(rows_operand(weight)) {
+    TORCH_CHECK(h.is_cuda() && h.scalar_type() == at::kBFloat16 && w.is_cuda() && w.scalar_type() == at::kBFloat16,
+                "linear head: bf16 CUDA tensors");
     T = h.size(0);
     H = h.size(1);
     V = w.size(0);
-    TORCH_CHECK(w.size(1) == H && w.get_device() == h.get_device(), "linear head: hidden [T, H] and weight [V, H]");
+    TORCH_CHECK(w.dim() == 2 && w.size(1) == H && w.get_device() == h.get_device(),
+                "linear head: hidden [T, H] and weight [V, H]");
     TORCH_CHECK(H > 0 && H % 8 == 0 && V > 0, "linear head: H must be a multiple of 8, V at least 1");
     TORCH_CHECK(T < INT_MAX / 2 && V < INT_MAX / 2, "linear head: too many rows");
     dev = h.get_device();
     stream = at::cuda::getCurrentCUDAStream(dev);
-    f32 = h.options().dtype(at::kFloat);
-    i32 = h.options().dtype(at::kInt);
   }
-  int64_t ldg() const { return round_up(V, kTile); }
-  int n_tiles() const { return static_cast<int>(ldg() / kTile); }
+  int64_t ldg() const { return round_up(V, kPad); }
   // Tokens per chunk: as many as `bytes` of 16-bit G hold (at least 256), spread evenly, in multiples of 256.
   int64_t chunk(int64_t bytes) const {
     const int64_t fit = std::max<int64_t>(256, bytes / (ldg() * 2) / 256 * 256);
     const int64_t n = (T + fit - 1) / fit;
     return n > 1 ? round_up((T + n - 1) / n, 256) : std::max<int64_t>(T, 1);
   }
-  at::Tensor gather(const at::Tensor& map, const at::Tensor& count) const {
-    // Up to 64 rows exist even for fewer tokens: the weight gradient's last K block reads them.
-    const int64_t rows = round_up(T, 64);
-    auto x = at::empty({rows, H}, h.options());
-    head_gather_kernel<<<static_cast<unsigned>(rows), H >= 1024 ? 128 : 64, 0, stream>>>(
-        reinterpret_cast<const bf16*>(h.data_ptr()), h.stride(0), static_cast<int>(H), static_cast<int>(T),
-        map.data_ptr<int>(), count.data_ptr<int>(), reinterpret_cast<bf16*>(x.data_ptr()));
-    NTB_LAUNCH_CHECK(1);
-    return x;
+};
+
+// The arrays of StateView in one int32 buffer.
+struct State {
+  at::Tensor buf;
+  StateView v;
+  int K;
+  bool distill;
+
+  static int64_t layout(int64_t T, int64_t K, bool distill, int64_t (&off)[11]) {
+    const int64_t TK = T * K;
+    const int64_t n[11] = {16, TK, T, T, T, T, TK, distill ? 0 : T, distill ? T : 0, distill ? TK : 0, distill ? T : 0};
+    int64_t at = 0;
+    for (int i = 0; i < 11; ++i) {
+      off[i] = at;
+      at += round_up(n[i], 4);
+    }
+    return at;
+  }
+  State(const Head& hd, int64_t K_, bool distill_, at::Tensor buf_ = {}) : buf(buf_), K(static_cast<int>(K_)), distill(distill_) {
+    int64_t off[11];
+    const int64_t ints = layout(hd.T, K, distill, off);
+    if (!buf.defined()) buf = at::empty({ints}, hd.h.options().dtype(at::kInt));
+    TORCH_CHECK(buf.is_cuda() && buf.scalar_type() == at::kInt && buf.is_contiguous() && buf.numel() == ints &&
+                    buf.get_device() == hd.dev,
+                "linear head: the state of another call");
+    int* p = buf.data_ptr<int>();
+    auto f = [&](int i) { return reinterpret_cast<float*>(p + off[i]); };
+    v = {reinterpret_cast<Header*>(p), p + off[1], p + off[2], p + off[3], f(4), f(5), f(6), f(7), p + off[8], f(9), f(10)};
   }
 };
 
-struct Targets {
-  at::Tensor targets, map, place, count, q, constant;
-  int K = 1;
-};
+// Gathers the live tokens. dh: rows of the others are zeroed (first pass only).
+at::Tensor gather(const Head& hd, const State& st, const int64_t* labels, int64_t vstart, int64_t ignore_index,
+                  bool mean, float* loss, float scale2, bf16* dh, bool known) {
+  auto x = at::empty({round_up(hd.T, 64), hd.H}, hd.h.options());
+  GatherParams p{};
+  p.h = reinterpret_cast<const bf16*>(hd.h.data_ptr());
+  p.ldh = hd.h.stride(0);
+  p.w = reinterpret_cast<const bf16*>(hd.w.data_ptr());
+  p.ldw = hd.w.stride(0);
+  p.H = static_cast<int>(hd.H);
+  p.T = static_cast<int>(hd.T);
+  p.labels = labels;
+  p.vstart = vstart;
+  p.V = hd.V;
+  p.ignore_index = ignore_index;
+  p.mean = mean ? 1 : 0;
+  p.scale2 = scale2;
+  p.st = st.v;
+  p.st.loss = loss;
+  p.x = reinterpret_cast<bf16*>(x.data_ptr());
+  p.dh = dh;
+  // 16 tokens a CTA; more from 65536 on, so that the counting reads T labels at most 4096 times.
+  p.tokens = static_cast<int>(std::max<int64_t>(16, round_up((hd.T + 4095) / 4096, 32)));
+  const unsigned blocks = static_cast<unsigned>((hd.T + p.tokens - 1) / p.tokens);
+  if (known) head_gather_kernel<true><<<blocks, kGatherThreads, 0, hd.stream>>>(p);
+  else head_gather_kernel<false><<<blocks, kGatherThreads, 0, hd.stream>>>(p);
+  NTB_LAUNCH_CHECK(1);
+  return x;
+}
 
-// Gradients of a chunk from its G: dH rows into `dh`, dW into `dw` (overwritten by the first chunk, then added to).
-void chunk_grads(const Head& hd, const at::Tensor& x, const at::Tensor& g, const Targets& t, int64_t c0, int64_t rows,
-                 at::Tensor* dh, at::Tensor* dw, bool first) {
+// Gradients of a chunk from its G: dH rows into `dh`, dW into `dw` (overwritten by the first chunk, then added to),
+// both times alpha (* *alpha_dev).
+void chunk_grads(const Head& hd, const at::Tensor& x, const at::Tensor& g, const State& st, int64_t c0, int64_t rows,
+                 double alpha, const float* alpha_dev, at::Tensor* dh, at::Tensor* dw, bool first, bool zero_others) {
   GemmTokenRows tok;
-  tok.rows = t.count.data_ptr<int>();
+  tok.rows = &st.v.head->count;
   tok.rows_base = static_cast<int>(c0);
   auto gv = g.narrow(0, 0, rows).narrow(1, 0, hd.V);
   if (dh) {
     tok.splits = pick_slices(rows, hd.H, hd.V, num_sms(hd.dev));
     tok.slice_stride = rows * hd.H;
-    auto part = at::empty({tok.splits, rows, hd.H}, hd.f32);
-    auto out = part.select(0, 0);
+    auto part = at::empty({tok.splits * rows, hd.H}, hd.h.options().dtype(at::kFloat));
+    auto out = part.narrow(0, 0, rows);
     gemm_bf16_tokens(gv, hd.w, out, false, true, false, tok);
-    head_dh_kernel<<<static_cast<unsigned>(hd.T), 256, 0, hd.stream>>>(
+    head_dh_kernel<<<static_cast<unsigned>(hd.T), hd.H >= 512 ? 256 : 64, 0, hd.stream>>>(
         part.data_ptr<float>(), tok.splits, static_cast<long>(tok.slice_stride), static_cast<int>(hd.H),
-        t.place.data_ptr<int>(), static_cast<int>(c0), static_cast<int>(c0 + rows), first ? 1 : 0,
-        reinterpret_cast<bf16*>(dh->data_ptr()));
+        static_cast<float>(alpha), alpha_dev, st.v.place, static_cast<int>(c0), static_cast<int>(c0 + rows),
+        first && zero_others ? 1 : 0, reinterpret_cast<bf16*>(dh->data_ptr()));
     NTB_LAUNCH_CHECK(1);
   }
   if (dw) {
     tok.splits = 1;
     tok.slice_stride = 0;
     tok.rows_are_k = true;
+    tok.alpha = alpha;
+    tok.alpha_dev = alpha_dev;
     gemm_bf16_tokens(gv, x.narrow(0, c0, rows), *dw, true, true, !first, tok);
   }
 }
 
-HeadParams logits_params(const Head& hd, const Targets& t, int64_t c0, int64_t rows, double inv_tau) {
+HeadParams logits_params(const Head& hd, const State& st, int64_t c0, int64_t rows, double tau) {
   HeadParams p{};
   p.M = static_cast<int>(rows);
   p.N = static_cast<int>(hd.V);
@@ -740,160 +865,90 @@ HeadParams logits_params(const Head& hd, const Targets& t, int64_t c0, int64_t r
   p.splits = 1;
   p.groups = 1;
   p.status = device_status(hd.dev);
-  p.rows = t.count.data_ptr<int>();
+  p.rows = &st.v.head->count;
   p.rows_base = static_cast<int>(c0);
-  p.scale2 = static_cast<float>(inv_tau * 1.4426950408889634);
-  p.map = t.map.data_ptr<int>() + c0;
-  p.targets = t.targets.data_ptr<int>();
-  p.n_targets = t.K;
-  p.n_tiles = hd.n_tiles();
+  p.scale2 = static_cast<float>(1.4426950408889634 / tau);
+  p.map = st.v.map + c0;
+  p.targets = st.v.targets;
+  p.n_targets = st.K;
+  p.picked = st.v.picked + c0 * st.K;
+  p.n_tiles = static_cast<int>(2 * ((hd.V + logits_tile(rows) - 1) / logits_tile(rows)));
   p.ldg = hd.ldg();
   return p;
 }
 
-RowParams row_params(const Head& hd, const Targets& t, int64_t c0) {
+RowParams row_params(const Head& hd, const State& st, int64_t c0) {
   RowParams p{};
-  p.rows = t.count.data_ptr<int>();
+  p.head = st.v.head;
   p.rows_base = static_cast<int>(c0);
-  p.map = t.map.data_ptr<int>() + c0;
-  p.targets = t.targets.data_ptr<int>();
-  p.q = t.q.defined() ? t.q.data_ptr<float>() : nullptr;
-  p.constant = t.constant.defined() ? t.constant.data_ptr<float>() : nullptr;
-  p.K = t.K;
-  p.n_tiles = hd.n_tiles();
+  p.map = st.v.map + c0;
+  p.targets = st.v.targets;
+  p.q = st.distill ? st.v.q : nullptr;
+  p.constant = st.distill ? st.v.constant : nullptr;
+  p.K = st.K;
+  p.picked = st.v.picked + c0 * st.K;
+  p.exact = st.distill ? nullptr : st.v.exact + c0;
+  p.lse2 = st.v.lse2 + c0;
   p.ldg = hd.ldg();
   p.V = static_cast<int>(hd.V);
   return p;
 }
 
-// Zero-token and bookkeeping arrays shared by both targets.
-void make_rows(const Head& hd, Targets& t, const int64_t* labels, int64_t vstart, int64_t ignore_index,
-               at::Tensor& loss) {
-  t.map = at::empty({std::max<int64_t>(1, hd.T)}, hd.i32);
-  t.place = at::empty({std::max<int64_t>(1, hd.T)}, hd.i32);
-  t.count = at::empty({1}, hd.i32);
-  head_rows_kernel<<<1, 1024, 0, hd.stream>>>(labels, vstart, hd.V, ignore_index, t.targets.data_ptr<int>(), t.K,
-                                              static_cast<int>(hd.T), t.map.data_ptr<int>(), t.place.data_ptr<int>(),
-                                              t.count.data_ptr<int>(), loss.data_ptr<float>());
-  NTB_LAUNCH_CHECK(1);
-}
-
 enum Reduction { kMean = 0, kSum = 1, kNone = 2 };
 
-// Returns {loss (scalar or [T]), loss rows, lse2, picked, targets, map, place, count, q, constant, dh, dw}.
-std::vector<at::Tensor> head_forward(const Head& hd, Targets& t, at::Tensor loss_rows, int64_t reduction, double tau,
-                                     bool need_dh, bool need_dw, bool dw_f32, int64_t bytes) {
-  const bool grads = need_dh || need_dw;
+struct ForwardOut {
+  at::Tensor loss, state, dh, dw;
+};
+
+// a: labels [T] int64, or the teacher's values [T, K] with b its indices.
+ForwardOut head_forward(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& a, const at::Tensor& b,
+                        double tau, int64_t ignore_index, int64_t reduction, int64_t vstart, int64_t bytes,
+                        bool need_dh, bool need_dw, bool dw_f32) {
+  const c10::cuda::CUDAGuard guard(hidden.device());
+  const Head hd(hidden, weight);
+  const bool distill = b.defined(), grads = need_dh || need_dw;
+  TORCH_CHECK(a.is_cuda() && a.get_device() == hd.dev && a.size(0) == hd.T, "linear head: targets of every token");
   TORCH_CHECK(!grads || reduction != kNone, "linear head: per-token losses take their gradient in the backward pass");
-  auto out = at::empty({}, hd.f32);
-  auto lse2 = at::empty({hd.T}, hd.f32);
-  auto picked = at::empty({hd.T, t.K}, hd.f32);
-  at::Tensor dh, dw;
-  const int64_t rows_max = hd.chunk(bytes);
-  if (need_dh) dh = at::empty({hd.T, hd.H}, hd.h.options());
-  if (need_dw) {
-    const bool several = rows_max < hd.T;
-    dw = at::empty({hd.V, hd.H}, hd.h.options().dtype(dw_f32 || several ? at::kFloat : at::kBFloat16));
-  }
-  if (hd.T == 0) {
-    out.zero_();
-    if (need_dw) dw.zero_();
+  if (distill) {
+    TORCH_CHECK(b.is_cuda() && b.get_device() == hd.dev && a.dim() == 2 && b.dim() == 2 && a.sizes() == b.sizes() &&
+                    a.stride(1) == 1 && b.stride(1) == 1 && a.size(1) >= 1 && a.size(1) <= 1024 && tau > 0,
+                "linear_distillation: teacher values and indices [T, K], K up to 1024, positive temperature");
   } else {
-    auto x = hd.gather(t.map, t.count);
-    auto part = at::empty({rows_max, hd.n_tiles(), 2}, hd.f32);
-    at::Tensor g;
-    // 64 rows at least: the weight gradient's last K block reads whole multiples of 64.
-    if (grads) g = at::empty({round_up(rows_max, 64), hd.ldg()}, hd.h.options());
-    for (int64_t c0 = 0; c0 < hd.T; c0 += rows_max) {
-      const int64_t rows = std::min(rows_max, hd.T - c0);
-      HeadParams p = logits_params(hd, t, c0, rows, 1.0 / tau);
-      p.picked = picked.data_ptr<float>() + c0 * t.K;
-      p.part = reinterpret_cast<float2*>(part.data_ptr<float>());
-      RowParams r = row_params(hd, t, c0);
-      r.picked = p.picked;
-      r.part = p.part;
-      r.loss = loss_rows.data_ptr<float>();
-      r.lse2 = lse2.data_ptr<float>() + c0;
-      r.loss_scale = static_cast<float>(tau * tau);
-      r.grad_scale = static_cast<float>(tau);
-      r.mean = reduction == kMean ? 1 : 0;
-      auto xc = x.narrow(0, c0, rows);
-      if (!grads) {
-        launch_logits<kStats>(xc, hd.w, p, hd.stream);
-        head_row_kernel<false><<<static_cast<unsigned>(rows), kRowThreads, 0, hd.stream>>>(r);
-        NTB_LAUNCH_CHECK(1);
-        continue;
-      }
-      p.codes = r.codes = reinterpret_cast<uint16_t*>(g.data_ptr());
-      launch_logits<kCodes>(xc, hd.w, p, hd.stream);
-      const size_t smem = static_cast<size_t>(hd.n_tiles()) * sizeof(float);
-      const int64_t rows64 = round_up(rows, 64);
-      head_row_kernel<true><<<static_cast<unsigned>(rows64), kRowThreads, smem, hd.stream>>>(r);
-      NTB_LAUNCH_CHECK(1);
-      chunk_grads(hd, x, g, t, c0, rows, need_dh ? &dh : nullptr, need_dw ? &dw : nullptr, c0 == 0);
-    }
-    if (reduction != kNone) {
-      head_loss_kernel<<<1, 1024, 0, hd.stream>>>(loss_rows.data_ptr<float>(), static_cast<int>(hd.T),
-                                                  t.count.data_ptr<int>(), reduction == kMean ? 1 : 0,
-                                                  out.data_ptr<float>());
-      NTB_LAUNCH_CHECK(1);
-    }
+    TORCH_CHECK(a.dim() == 1 && a.scalar_type() == at::kLong && a.is_contiguous(),
+                "linear_cross_entropy: contiguous int64 labels");
   }
-  return {reduction == kNone ? loss_rows : out, lse2, picked, t.targets, t.map, t.place, t.count, t.q, t.constant,
-          dh, dw};
-}
-
-}  // namespace
-
-std::vector<at::Tensor> linear_ce_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& labels,
-                                      int64_t vstart, int64_t ignore_index, int64_t reduction, bool need_dh,
-                                      bool need_dw, bool dw_f32, int64_t bytes) {
-  const c10::cuda::CUDAGuard guard(hidden.device());
-  Head hd(hidden, weight);
-  TORCH_CHECK(labels.is_cuda() && labels.scalar_type() == at::kLong && labels.dim() == 1 && labels.is_contiguous() &&
-                  labels.size(0) == hd.T && labels.get_device() == hd.dev,
-              "linear_cross_entropy: int64 labels, one for each token");
-  Targets t;
-  t.targets = at::empty({std::max<int64_t>(1, hd.T)}, hd.i32);
-  auto loss_rows = at::empty({hd.T}, hd.f32);
-  make_rows(hd, t, labels.data_ptr<int64_t>(), vstart, ignore_index, loss_rows);
-  return head_forward(hd, t, loss_rows, reduction, 1.0, need_dh, need_dw, dw_f32, bytes);
-}
-
-std::vector<at::Tensor> linear_distill_fwd(const at::Tensor& hidden, const at::Tensor& weight,
-                                           const at::Tensor& values, const at::Tensor& indices, double tau,
-                                           int64_t reduction, bool need_dh, bool need_dw, bool dw_f32,
-                                           int64_t bytes) {
-  const c10::cuda::CUDAGuard guard(hidden.device());
-  Head hd(hidden, weight);
-  TORCH_CHECK(values.is_cuda() && indices.is_cuda() && values.dim() == 2 && indices.dim() == 2 &&
-                  values.size(0) == hd.T && indices.size(0) == hd.T && values.size(1) == indices.size(1) &&
-                  values.stride(1) == 1 && indices.stride(1) == 1 && values.get_device() == hd.dev &&
-                  indices.get_device() == hd.dev,
-              "linear_distillation: teacher values and indices [T, K] with unit inner stride");
-  const int64_t K = values.size(1);
-  TORCH_CHECK(K >= 1 && K <= 1024, "linear_distillation: 1 to 1024 teacher logits a token");
-  TORCH_CHECK(tau > 0, "linear_distillation: positive temperature");
-  Targets t;
-  t.K = static_cast<int>(K);
-  t.targets = at::empty({std::max<int64_t>(1, hd.T), K}, hd.i32);
-  t.q = at::empty({hd.T, K}, hd.f32);
-  t.constant = at::empty({hd.T}, hd.f32);
-  auto loss_rows = at::empty({hd.T}, hd.f32);
-  if (hd.T > 0) {
+  State st(hd, distill ? a.size(1) : 1, distill);
+  const auto f32 = hd.h.options().dtype(at::kFloat);
+  const int64_t rows_max = hd.chunk(bytes);
+  ForwardOut out;
+  out.state = st.buf;
+  if (reduction == kNone) {
+    auto lead = hidden.sizes().vec();
+    lead.pop_back();
+    out.loss = at::empty(lead, f32);
+  } else {
+    out.loss = at::empty({}, f32);
+  }
+  if (need_dh) out.dh = at::empty(hidden.sizes(), hd.h.options());
+  if (need_dw) out.dw = at::empty({hd.V, hd.H}, dw_f32 || rows_max < hd.T ? f32 : hd.h.options());
+  if (hd.T == 0) {
+    if (reduction != kNone) out.loss.zero_();
+    if (need_dw) out.dw.zero_();
+    return out;
+  }
+  if (distill) {
     int P = 32;
-    while (P < K) P *= 2;
+    while (P < st.K) P *= 2;
     const int threads = std::min(256, std::max(32, P / 2));
     const size_t smem = static_cast<size_t>(P) * 8;
     auto launch = [&](auto vt, auto it) {
       using VT = decltype(vt);
       using IT = decltype(it);
       head_teacher_kernel<VT, IT><<<static_cast<unsigned>(hd.T), threads, smem, hd.stream>>>(
-          reinterpret_cast<const VT*>(values.data_ptr()), values.stride(0),
-          reinterpret_cast<const IT*>(indices.data_ptr()), indices.stride(0), t.K, P, static_cast<float>(1.0 / tau),
-          hd.V, t.targets.data_ptr<int>(), t.q.data_ptr<float>(), t.constant.data_ptr<float>());
+          reinterpret_cast<const VT*>(a.data_ptr()), a.stride(0), reinterpret_cast<const IT*>(b.data_ptr()),
+          b.stride(0), st.K, P, static_cast<float>(1.0 / tau), hd.V, st.v.targets, st.v.live, st.v.q, st.v.constant);
     };
-    const auto vs = values.scalar_type(), is = indices.scalar_type();
+    const auto vs = a.scalar_type(), is = b.scalar_type();
     TORCH_CHECK(is == at::kLong || is == at::kInt, "linear_distillation: int64 or int32 indices");
     auto by_index = [&](auto vt) {
       if (is == at::kLong) launch(vt, int64_t{});
@@ -905,93 +960,102 @@ std::vector<at::Tensor> linear_distill_fwd(const at::Tensor& hidden, const at::T
     else TORCH_CHECK(false, "linear_distillation: fp32, bf16 or fp16 teacher values");
     NTB_LAUNCH_CHECK(1);
   }
-  make_rows(hd, t, nullptr, 0, 0, loss_rows);
-  return head_forward(hd, t, loss_rows, reduction, tau, need_dh, need_dw, dw_f32, bytes);
+  float* loss = reduction == kNone ? out.loss.data_ptr<float>() : st.v.loss;
+  const float scale2 = static_cast<float>(1.4426950408889634 / tau);
+  auto x = gather(hd, st, distill ? nullptr : a.data_ptr<int64_t>(), vstart, ignore_index, reduction == kMean, loss,
+                  scale2, need_dh ? reinterpret_cast<bf16*>(out.dh.data_ptr()) : nullptr, false);
+  auto part = at::empty({rows_max, hd.ldg() / (logits_tile(rows_max) / 2), 2}, f32);
+  at::Tensor g;
+  // 64 rows at least: the weight gradient's last K block reads whole multiples of 64.
+  if (grads) g = at::empty({round_up(rows_max, 64), hd.ldg()}, hd.h.options());
+  int tickets = 0;
+  for (int64_t c0 = 0; c0 < hd.T; c0 += rows_max) {
+    const int64_t rows = std::min(rows_max, hd.T - c0);
+    tickets += static_cast<int>(grads ? round_up(rows, 64) : rows);
+  }
+  for (int64_t c0 = 0; c0 < hd.T; c0 += rows_max) {
+    const int64_t rows = std::min(rows_max, hd.T - c0);
+    HeadParams p = logits_params(hd, st, c0, rows, tau);
+    p.part = reinterpret_cast<float2*>(part.data_ptr<float>());
+    RowParams r = row_params(hd, st, c0);
+    r.part = p.part;
+    r.n_tiles = p.n_tiles;
+    r.tile_shift = logits_tile(rows) == 256 ? 4 : 3;
+    r.loss = loss;
+    r.loss_scale = static_cast<float>(tau * tau);
+    if (reduction != kNone) {
+      r.ticket = &st.v.head->ticket;
+      r.tickets = tickets;
+      r.T = static_cast<int>(hd.T);
+      r.out = out.loss.data_ptr<float>();
+    }
+    auto xc = x.narrow(0, c0, rows);
+    if (!grads) {
+      launch_logits<kStats>(xc, hd.w, p, hd.stream);
+      head_row_kernel<false><<<static_cast<unsigned>(rows), kRowThreads, 0, hd.stream>>>(r);
+      NTB_LAUNCH_CHECK(1);
+      continue;
+    }
+    p.codes = r.codes = reinterpret_cast<uint16_t*>(g.data_ptr());
+    launch_logits<kCodes>(xc, hd.w, p, hd.stream);
+    head_row_kernel<true><<<static_cast<unsigned>(round_up(rows, 64)), kRowThreads,
+                            static_cast<size_t>(p.n_tiles) * sizeof(float), hd.stream>>>(r);
+    NTB_LAUNCH_CHECK(1);
+    chunk_grads(hd, x, g, st, c0, rows, tau, &st.v.head->inv, need_dh ? &out.dh : nullptr,
+                need_dw ? &out.dw : nullptr, c0 == 0, false);
+  }
+  return out;
 }
 
-// Gradients with the statistics of the forward pass known: G = (p - q) tau row_scale[token].
-// Returns {dh, dw}; dw is fp32 when asked for or when the tokens take several chunks.
-std::vector<at::Tensor> linear_head_bwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& lse2,
-                                        const at::Tensor& picked, const at::Tensor& targets, const at::Tensor& map,
-                                        const at::Tensor& place, const at::Tensor& count,
-                                        const c10::optional<at::Tensor>& q, const at::Tensor& row_scale, double tau,
-                                        bool need_dh, bool need_dw, bool dw_f32, int64_t bytes) {
+// Gradients with the statistics of the forward pass known: G = (p - q) tau row_scale[token]. dw is fp32 when asked
+// for or when the tokens take several chunks.
+std::pair<at::Tensor, at::Tensor> head_backward(const at::Tensor& hidden, const at::Tensor& weight,
+                                                const at::Tensor& state, int64_t K, bool distill,
+                                                const at::Tensor& row_scale, double tau, bool need_dh, bool need_dw,
+                                                bool dw_f32, int64_t bytes) {
   const c10::cuda::CUDAGuard guard(hidden.device());
-  Head hd(hidden, weight);
+  const Head hd(hidden, weight);
+  const State st(hd, K, distill, state);
   TORCH_CHECK(row_scale.is_cuda() && row_scale.scalar_type() == at::kFloat && row_scale.is_contiguous() &&
                   row_scale.numel() == hd.T,
               "linear head: one fp32 gradient for each token");
-  Targets t;
-  t.targets = targets;
-  t.map = map;
-  t.place = place;
-  t.count = count;
-  if (q.has_value() && q->defined()) t.q = *q;
-  t.K = static_cast<int>(picked.size(1));
   at::Tensor dh, dw;
   const int64_t rows_max = hd.chunk(bytes);
-  if (need_dh) dh = at::empty({hd.T, hd.H}, hd.h.options());
-  if (need_dw) dw = at::empty({hd.V, hd.H}, hd.h.options().dtype(dw_f32 || rows_max < hd.T ? at::kFloat : at::kBFloat16));
+  if (need_dh) dh = at::empty(hidden.sizes(), hd.h.options());
+  if (need_dw)
+    dw = at::empty({hd.V, hd.H}, dw_f32 || rows_max < hd.T ? hd.h.options().dtype(at::kFloat) : hd.h.options());
   if (hd.T == 0) {
     if (need_dw) dw.zero_();
     return {dh, dw};
   }
-  auto x = hd.gather(t.map, t.count);
+  auto x = gather(hd, st, nullptr, 0, 0, false, nullptr, 0.f, nullptr, true);
   auto g = at::empty({round_up(rows_max, 64), hd.ldg()}, hd.h.options());
   for (int64_t c0 = 0; c0 < hd.T; c0 += rows_max) {
     const int64_t rows = std::min(rows_max, hd.T - c0);
-    HeadParams p = logits_params(hd, t, c0, rows, 1.0 / tau);
-    p.lse2 = lse2.data_ptr<float>() + c0;
+    HeadParams p = logits_params(hd, st, c0, rows, tau);
+    p.lse2 = st.v.lse2 + c0;
     p.row_scale = row_scale.data_ptr<float>();
     p.grad_scale = static_cast<float>(tau);
     p.codes = reinterpret_cast<uint16_t*>(g.data_ptr());
     launch_logits<kGrad>(x.narrow(0, c0, rows), hd.w, p, hd.stream);
-    RowParams r = row_params(hd, t, c0);
-    r.picked = picked.data_ptr<float>() + c0 * t.K;
-    r.lse2 = const_cast<float*>(p.lse2);
+    RowParams r = row_params(hd, st, c0);
     r.codes = p.codes;
     r.grad_scale = p.grad_scale;
-    head_fix_kernel<<<static_cast<unsigned>(round_up(rows, 64)), t.K >= 128 ? 128 : 64, 0, hd.stream>>>(
+    head_fix_kernel<<<static_cast<unsigned>(round_up(rows, 64)), st.K >= 128 ? 128 : 64, 0, hd.stream>>>(
         r, row_scale.data_ptr<float>());
     NTB_LAUNCH_CHECK(1);
-    chunk_grads(hd, x, g, t, c0, rows, need_dh ? &dh : nullptr, need_dw ? &dw : nullptr, c0 == 0);
+    chunk_grads(hd, x, g, st, c0, rows, 1.0, nullptr, need_dh ? &dh : nullptr, need_dw ? &dw : nullptr, c0 == 0, true);
   }
   return {dh, dw};
 }
 
-// x *= factor (a device scalar), in place; bf16 or fp32.
-void head_scale_(at::Tensor& x, const at::Tensor& factor) {
-  const c10::cuda::CUDAGuard guard(x.device());
-  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && factor.is_cuda() && factor.scalar_type() == at::kFloat &&
-                  factor.numel() == 1,
-              "head_scale_: contiguous CUDA tensor and fp32 factor");
-  const int64_t n = x.numel();
-  if (n == 0) return;
-  auto stream = at::cuda::getCurrentCUDAStream();
-  const int blocks = stream_blocks(n, 256 * 8);
-  if (x.scalar_type() == at::kBFloat16)
-    head_scale_kernel<bf16><<<blocks, 256, 0, stream>>>(reinterpret_cast<bf16*>(x.data_ptr()), n,
-                                                        factor.data_ptr<float>());
-  else {
-    TORCH_CHECK(x.scalar_type() == at::kFloat, "head_scale_: bf16 or fp32");
-    head_scale_kernel<float><<<blocks, 256, 0, stream>>>(x.data_ptr<float>(), n, factor.data_ptr<float>());
-  }
-  NTB_LAUNCH_CHECK(1);
-}
-
 // dst = (accumulate: dst +) factor * src; src fp32, dst bf16 or fp32 (accumulate: fp32). factor: device scalar or none.
-void head_scaled_copy_(const at::Tensor& src, const c10::optional<at::Tensor>& factor, at::Tensor& dst,
-                       bool accumulate) {
-  const c10::cuda::CUDAGuard guard(src.device());
-  TORCH_CHECK(src.is_cuda() && dst.is_cuda() && src.scalar_type() == at::kFloat && src.is_contiguous() &&
-                  dst.is_contiguous() && src.numel() == dst.numel() && (!accumulate || dst.scalar_type() == at::kFloat),
-              "head_scaled_copy_: fp32 source, contiguous destination of the same size");
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(dst.data_ptr()) & 15) == 0, "head_scaled_copy_: 16-byte aligned destination");
+void scaled_copy(const at::Tensor& src, const at::Tensor& factor, at::Tensor& dst, bool accumulate) {
   const int64_t n = src.numel();
   if (n == 0) return;
-  const float* f = factor.has_value() ? factor->data_ptr<float>() : nullptr;
+  const float* f = factor.defined() ? factor.data_ptr<float>() : nullptr;
   auto stream = at::cuda::getCurrentCUDAStream();
-  const int blocks = stream_blocks(n, 256 * 4);
+  const unsigned blocks = stream_blocks(n, 256 * 4);
   const float* s = src.data_ptr<float>();
   if (dst.scalar_type() == at::kBFloat16)
     head_scaled_copy_kernel<bf16, false><<<blocks, 256, 0, stream>>>(s, n, f, reinterpret_cast<bf16*>(dst.data_ptr()));
@@ -1000,6 +1064,148 @@ void head_scaled_copy_(const at::Tensor& src, const c10::optional<at::Tensor>& f
   else
     head_scaled_copy_kernel<float, false><<<blocks, 256, 0, stream>>>(s, n, f, dst.data_ptr<float>());
   NTB_LAUNCH_CHECK(1);
+}
+
+// The ready gradients times the upstream gradient: dh and a bf16 dw in place, an fp32 dw into bf16.
+void finish_grads(at::Tensor& dh, at::Tensor& dw, const at::Tensor& factor) {
+  const bool half_dw = dw.defined() && dw.scalar_type() == at::kBFloat16;
+  const int64_t na = dh.defined() ? dh.numel() : 0, nb = half_dw ? dw.numel() : 0;
+  if (na + nb > 0) {
+    head_scale_kernel<<<stream_blocks(na + nb, 256 * 8), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
+        na ? reinterpret_cast<bf16*>(dh.data_ptr()) : nullptr, na,
+        nb ? reinterpret_cast<bf16*>(dw.data_ptr()) : nullptr, nb, factor.data_ptr<float>());
+    NTB_LAUNCH_CHECK(1);
+  }
+  if (dw.defined() && !half_dw) {
+    auto out = at::empty(dw.sizes(), dw.options().dtype(at::kBFloat16));
+    scaled_copy(dw, factor, out, false);
+    dw = out;
+  }
+}
+
+// Autograd node of the usual case (no main_grad, no shards). It lives here because the backward pass of a small head
+// is bound by the host: a node in Python adds 30 us of interpreter and lock hand-over to each step.
+class HeadLoss : public torch::autograd::Function<HeadLoss> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden, const at::Tensor& weight,
+                            const at::Tensor& a, const c10::optional<at::Tensor>& b_or, double tau,
+                            int64_t ignore_index, int64_t reduction, int64_t vstart, int64_t bytes, bool need_dh,
+                            bool need_dw) {
+    const at::Tensor b = b_or.has_value() ? *b_or : at::Tensor();
+    const bool now = reduction != kNone;
+    auto out = head_forward(hidden, weight, a, b, tau, ignore_index, reduction, vstart, bytes, now && need_dh,
+                            now && need_dw, false);
+    if (need_dh || need_dw) {
+      ctx->save_for_backward({hidden, weight, out.state});
+      if (out.dh.defined()) ctx->saved_data["dh"] = out.dh;
+      if (out.dw.defined()) ctx->saved_data["dw"] = out.dw;
+      ctx->saved_data["ready"] = now;
+      ctx->saved_data["K"] = b.defined() ? b.size(1) : int64_t{0};
+      ctx->saved_data["tau"] = tau;
+      ctx->saved_data["mean"] = reduction == kMean;
+      ctx->saved_data["bytes"] = bytes;
+      ctx->saved_data["need"] = (need_dh ? 1 : 0) + (need_dw ? 2 : 0);
+    }
+    return out.loss;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 const torch::autograd::variable_list& grads) {
+    auto& d = ctx->saved_data;
+    const int64_t need = d["need"].toInt(), K = d["K"].toInt();
+    const auto saved = ctx->get_saved_variables();
+    const c10::cuda::CUDAGuard guard(saved[0].device());
+    at::Tensor dh, dw, gout = grads[0].scalar_type() == at::kFloat ? grads[0] : grads[0].to(at::kFloat);
+    if (d["ready"].toBool()) {
+      d["ready"] = false;  // handed on: a second backward pass computes them again
+      if (need & 1) dh = d["dh"].toTensor();
+      if (need & 2) dw = d["dw"].toTensor();
+      d.erase("dh");
+      d.erase("dw");
+      finish_grads(dh, dw, gout);
+    } else {
+      const at::Tensor& state = saved[2];
+      const int64_t T = saved[0].numel() / saved[0].size(-1);
+      if (gout.dim() == 0 && T > 0) {
+        if (d["mean"].toBool()) gout = gout * state.narrow(0, 2, 1).view(at::kFloat);  // Header::inv
+        gout = gout.expand({T});
+      }
+      std::tie(dh, dw) = head_backward(saved[0], saved[1], state, std::max<int64_t>(K, 1), K > 0,
+                                       gout.reshape({-1}).contiguous(), d["tau"].toDouble(), need & 1, need & 2, false,
+                                       d["bytes"].toInt());
+      if (dw.defined() && dw.scalar_type() != at::kBFloat16) {
+        auto half = at::empty(dw.sizes(), dw.options().dtype(at::kBFloat16));
+        scaled_copy(dw, {}, half, false);
+        dw = half;
+      }
+    }
+    torch::autograd::variable_list out(11);
+    out[0] = dh;
+    out[1] = dw;
+    return out;
+  }
+};
+
+at::Tensor or_undefined(const c10::optional<at::Tensor>& t) { return t.has_value() ? *t : at::Tensor(); }
+
+}  // namespace
+
+// hidden [..., H], weight [V, H]; a: labels [T], or the teacher's values [T, K] with b its indices.
+at::Tensor linear_head_loss(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& a,
+                            const c10::optional<at::Tensor>& b, double tau, int64_t ignore_index, int64_t reduction,
+                            int64_t vstart, int64_t bytes) {
+  const bool on = at::GradMode::is_enabled();
+  return HeadLoss::apply(hidden, weight, a, b, tau, ignore_index, reduction, vstart, bytes,
+                         on && hidden.requires_grad(), on && weight.requires_grad());
+}
+
+// The pieces, for callers that deliver the gradients themselves: {loss, state, dh, dw}.
+std::vector<at::Tensor> linear_head_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& a,
+                                        const c10::optional<at::Tensor>& b, double tau, int64_t ignore_index,
+                                        int64_t reduction, int64_t vstart, int64_t bytes, bool need_dh, bool need_dw,
+                                        bool dw_f32) {
+  auto out = head_forward(hidden, weight, a, or_undefined(b), tau, ignore_index, reduction, vstart, bytes, need_dh,
+                          need_dw, dw_f32);
+  return {out.loss, out.state, out.dh, out.dw};
+}
+
+// Views of a state: {count [1] int32, targets [T, K] int32, map [T] int32, lse2 [T], picked [T, K]}.
+std::vector<at::Tensor> linear_head_state(const at::Tensor& state, int64_t T, int64_t K, bool distill) {
+  int64_t off[11];
+  TORCH_CHECK(State::layout(T, K, distill, off) == state.numel(), "linear head: the state of another call");
+  auto f = [&](int i, int64_t n) { return state.narrow(0, off[i], n).view(at::kFloat); };
+  return {state.narrow(0, 0, 1), state.narrow(0, off[1], T * K).view({T, K}), state.narrow(0, off[2], T), f(5, T),
+          f(6, T * K).view({T, K})};
+}
+
+std::vector<at::Tensor> linear_head_bwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& state,
+                                        int64_t K, bool distill, const at::Tensor& row_scale, double tau,
+                                        bool need_dh, bool need_dw, bool dw_f32, int64_t bytes) {
+  auto out = head_backward(hidden, weight, state, K, distill, row_scale, tau, need_dh, need_dw, dw_f32, bytes);
+  return {out.first, out.second};
+}
+
+// dh *= factor in place and dst += factor * dw (fp32 both), either of them optional.
+void linear_head_deliver_(const c10::optional<at::Tensor>& dh, const c10::optional<at::Tensor>& dw,
+                          const c10::optional<at::Tensor>& factor, const c10::optional<at::Tensor>& into) {
+  auto a = or_undefined(dh), none = at::Tensor(), f = or_undefined(factor);
+  TORCH_CHECK(!a.defined() || f.defined(), "linear head: a factor");
+  TORCH_CHECK(!f.defined() || (f.is_cuda() && f.scalar_type() == at::kFloat && f.numel() == 1), "linear head: fp32 factor");
+  if (a.defined()) {
+    const c10::cuda::CUDAGuard guard(a.device());
+    TORCH_CHECK(a.is_cuda() && a.scalar_type() == at::kBFloat16 && a.is_contiguous(), "linear head: bf16 gradient");
+    finish_grads(a, none, f);
+  }
+  if (dw.has_value() && dw->defined()) {
+    TORCH_CHECK(into.has_value(), "linear head: a gradient buffer");
+    at::Tensor dst = *into;
+    const c10::cuda::CUDAGuard guard(dst.device());
+    TORCH_CHECK(dw->is_cuda() && dw->scalar_type() == at::kFloat && dw->is_contiguous() && dst.is_cuda() &&
+                    dst.scalar_type() == at::kFloat && dst.is_contiguous() && dst.numel() == dw->numel() &&
+                    (reinterpret_cast<uintptr_t>(dst.data_ptr()) & 15) == 0,
+                "linear head: contiguous fp32 gradient buffer on a 16-byte boundary");
+    scaled_copy(*dw, f, dst, true);
+  }
 }
 
 }  // namespace ntb

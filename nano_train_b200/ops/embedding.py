@@ -52,6 +52,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, vocab_start: int = 0) -> 
 
 
 class _ScaledEmbeddingFn(torch.autograd.Function):
+    """Lookups whose weight carries a ``main_grad``; the others take the node of the extension."""
+
     @staticmethod
     def forward(ctx, ids, weight, scale, vstart):
         ctx.save_for_backward(ids)
@@ -63,13 +65,7 @@ class _ScaledEmbeddingFn(torch.autograd.Function):
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
         weight, scale, vstart = ctx.meta
-        ids, dout = ids.reshape(-1), dout.reshape(-1, weight.shape[1]).contiguous()
-        mg = getattr(weight, "main_grad", None)
-        if mg is None:
-            dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
-            ext().scaled_embedding_bwd(ids, dout, scale, vstart, dw, False)
-            return None, dw, None, None
-        ext().scaled_embedding_bwd(ids, dout, scale, vstart, mg, True)
+        ext().scaled_embedding_add_(ids, dout.contiguous(), scale, vstart, weight.main_grad)
         hook = getattr(weight, "_ntb_grad_ready_hook", None)
         if hook is not None:
             hook(weight)
@@ -93,7 +89,9 @@ def scaled_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0
     if weight.is_cuda:
         if weight.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError(f"scaled_embedding: CUDA weights must be bfloat16 or float32, got {weight.dtype}")
-        return _ScaledEmbeddingFn.apply(ids.contiguous(), weight, float(scale), vocab_start)
+        if getattr(weight, "main_grad", None) is not None:
+            return _ScaledEmbeddingFn.apply(ids.contiguous(), weight, float(scale), vocab_start)
+        return ext().scaled_embedding(ids.contiguous(), weight, float(scale), vocab_start)
     if not weight.dtype.is_floating_point:
         raise TypeError(f"scaled_embedding: floating weight expected, got {weight.dtype}")
     local = ids - vocab_start

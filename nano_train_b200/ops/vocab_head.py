@@ -21,7 +21,7 @@ logits); distillation has no counterpart there.
 """
 from __future__ import annotations
 
-from typing import Optional
+import math
 
 import torch
 import torch.distributed as dist
@@ -34,118 +34,87 @@ DEFAULT_WORKSPACE_MB = 2048
 MAX_TEACHER_LOGITS = 1024
 
 
-def _grad_buffer(weight) -> Optional[torch.Tensor]:
-    mg = getattr(weight, "main_grad", None)
-    return mg if mg is not None and mg.dtype == torch.float32 and mg.is_cuda and mg.is_contiguous() else None
-
-
-def _deliver_weight_grad(weight, dw, factor=None):
-    """dw (times a device scalar) into ``main_grad`` when the weight has one, else as the weight's gradient."""
-    if dw is None:
-        return None
-    mg = getattr(weight, "main_grad", None)
-    if mg is not None:
-        into = _grad_buffer(weight)
-        if into is not None and dw.dtype == torch.float32:
-            ext().head_scaled_copy_(dw, factor, into, True)
-        else:
-            mg.add_(dw if factor is None else dw * factor)
-        hook = getattr(weight, "_ntb_grad_ready_hook", None)
-        if hook is not None:
-            hook(weight)
-        return None
-    if dw.dtype == weight.dtype:
-        if factor is not None:
-            ext().head_scale_(dw, factor)
-        return dw
-    out = torch.empty_like(dw, dtype=weight.dtype)
-    ext().head_scaled_copy_(dw, factor, out, False)
-    return out
-
-
 def _world(group) -> int:
     return dist.get_world_size(group) if group is not None else 1
 
 
 class _HeadLossFn(torch.autograd.Function):
-    """Loss of a head over compacted tokens; ``labels`` or (``values``, ``indices``) are its targets."""
+    """Losses whose weight gradient goes into ``main_grad``, or whose vocabulary is sharded over ``group``; the
+    others take the node of the extension. ``targets`` are labels, or teacher values with ``indices``."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, labels, values, indices, tau, ignore_index, reduction, vstart, group, nbytes,
-                with_grad):
-        shape = hidden.shape
-        h = _rows_operand(hidden.reshape(-1, shape[-1]))
-        w = _rows_operand(weight)
+    def forward(ctx, hidden, weight, targets, indices, tau, ignore_index, reduction, vstart, group, nbytes, with_grad):
         sharded = _world(group) > 1
         need_dh = with_grad and ctx.needs_input_grad[0]
         need_dw = with_grad and ctx.needs_input_grad[1]
-        now = reduction != "none" and not sharded and (need_dh or need_dw)
-        red = _REDUCTIONS["none" if sharded else reduction]
-        dw_f32 = getattr(weight, "main_grad", None) is not None
-        if labels is not None:
-            out = ext().linear_ce_fwd(h, w, labels, vstart, ignore_index, red, now and need_dh, now and need_dw, dw_f32,
-                                      nbytes)
-        else:
-            out = ext().linear_distill_fwd(h, w, values, indices, tau, red, now and need_dh, now and need_dw, dw_f32,
-                                           nbytes)
-        loss, lse2, picked, targets, tmap, place, count, q, _constant, dh, dw = out
+        now = reduction != "none" and not sharded
+        main = getattr(weight, "main_grad", None) is not None
+        loss, state, dh, dw = ext().linear_head_fwd(
+            hidden, weight, targets, indices, tau, ignore_index, _REDUCTIONS["none" if sharded else reduction], vstart,
+            nbytes, now and need_dh, now and need_dw, main)
+        K = indices.shape[1] if indices is not None else 0
+        inv = None
         if sharded:
-            loss, lse2 = _join_shards(loss, lse2, picked, targets, tmap, count, reduction, group)
+            loss, inv = _join_shards(loss, state, reduction, group)
         if with_grad:
-            ctx.save_for_backward(h, w, lse2, picked, targets, tmap, place, count, q)
+            ctx.save_for_backward(hidden, weight, state, inv)
             ctx.ready = (dh, dw) if now else None
-            ctx.meta = (weight, shape, tau, reduction, group if sharded else None, nbytes, dw_f32)
-        return loss.view(shape[:-1]) if reduction == "none" else loss
+            ctx.meta = (weight, tau, K, reduction, group if sharded else None, nbytes, main)
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        weight, shape, tau, reduction, group, nbytes, dw_f32 = ctx.meta
-        need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        weight, tau, K, reduction, group, nbytes, main = ctx.meta
         gout = gout.float()
-        none = (None,) * 10
+        none = (None,) * 9
         if ctx.ready is not None:
             dh, dw = ctx.ready
             ctx.ready = None  # handed on: a second backward pass computes them again
-            factor = gout.reshape(1)
             if dh is not None:
-                ext().head_scale_(dh, factor)
-                dh = dh.view(shape)
-            return (dh, _deliver_weight_grad(weight, dw, factor), *none)
-        h, w, lse2, picked, targets, tmap, place, count, q = ctx.saved_tensors
+                ext().linear_head_deliver_(dh, None, gout, None)
+            return (dh, _deliver(weight, dw, gout), *none)
+        hidden, w, state, inv = ctx.saved_tensors
+        need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         if reduction == "none":
             scale = gout.reshape(-1).contiguous()
         else:
             if reduction == "mean":
-                gout = gout / count.clamp_min(1)
-            scale = gout.reshape(1).expand(h.shape[0]).contiguous()
-        dh, dw = ext().linear_head_bwd(h, w, lse2, picked, targets, tmap, place, count, q, scale, tau, need_dh, need_dw,
-                                       dw_f32, nbytes)
-        if dh is not None:
-            if group is not None:
-                dist.all_reduce(dh, group=group)
-            dh = dh.view(shape)
-        return (dh, _deliver_weight_grad(weight, dw), *none)
+                inv = inv if inv is not None else state[2:3].view(torch.float32)
+                gout = gout * inv
+            scale = gout.reshape(1).expand(hidden.numel() // hidden.shape[-1]).contiguous()
+        dh, dw = ext().linear_head_bwd(hidden, w, state, max(K, 1), K > 0, scale, tau, need_dh, need_dw, main, nbytes)
+        if dh is not None and group is not None:
+            dist.all_reduce(dh, group=group)
+        return (dh, _deliver(weight, dw), *none)
 
 
-def _rows_operand(t: torch.Tensor) -> torch.Tensor:
-    """A 2-D view the tensor maps take: unit inner stride, every row on a 16-byte boundary."""
-    if t.stride(-1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) and t.stride(0) % 8 == 0 \
-            and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _deliver(weight, dw, factor=None):
+    """dw (times a device scalar) into ``main_grad`` when the weight has one, else as the weight's gradient."""
+    if dw is None:
+        return None
+    mg = getattr(weight, "main_grad", None)
+    if mg is None:
+        return (dw if factor is None else dw * factor).to(weight.dtype)
+    if dw.dtype == torch.float32 and mg.dtype == torch.float32 and mg.is_contiguous() and mg.data_ptr() % 16 == 0:
+        ext().linear_head_deliver_(None, dw, factor, mg)
+    else:
+        mg.add_(dw if factor is None else dw * factor)
+    hook = getattr(weight, "_ntb_grad_ready_hook", None)
+    if hook is not None:
+        hook(weight)
+    return None
 
 
-def _join_shards(rows, lse2, picked, targets, tmap, count, reduction, group):
-    """Row losses over a vocabulary sharded across ``group``: lse and the label's logit are summed over the ranks.
-
-    ``rows`` is each rank's loss with the logits it has; log-sum-exp joins by (MAX, SUM), the label's logit, which
-    one rank has, by SUM. Statistics are in compact token order; rows past the device count are not read.
-    """
+def _join_shards(rows, state, reduction, group):
+    """Row losses over a vocabulary sharded across ``group``: log-sum-exp joins by (MAX, SUM) over the ranks, the
+    label's logit, which one rank has, by SUM. The statistics are in compact token order; rows past the count are
+    not read. The joined log-sum-exp replaces the rank's own in ``state``. Returns (loss, 1 / count)."""
     T = rows.numel()
+    count, targets, tmap, own_lse2, picked = ext().linear_head_state(state, T, 1, False)
     live = torch.arange(T, device=rows.device) < count
-    lse2 = torch.where(live, lse2, 0.0)
-    tok = torch.where(live, tmap[:T].long(), 0)
+    lse2 = torch.where(live, own_lse2, 0.0)
+    tok = torch.where(live, tmap.long(), 0)
     here = live & (targets.view(-1)[tok] != torch.iinfo(torch.int32).max)
     x2 = torch.where(here, picked[:, 0], 0.0)
     top = lse2.clone()
@@ -154,12 +123,23 @@ def _join_shards(rows, lse2, picked, targets, tmap, count, reduction, group):
     dist.all_reduce(total, group=group)
     dist.all_reduce(x2, group=group)
     lse2 = top + torch.log2(total)
-    value = torch.where(live, (lse2 - x2) * 0.6931471805599453, 0.0)
-    loss = torch.zeros_like(rows).index_add_(0, tok, value)
+    own_lse2.copy_(lse2)
+    value = torch.where(live, (lse2 - x2) * math.log(2.0), 0.0)
+    loss = torch.zeros(T, device=rows.device).index_add_(0, tok, value)
+    inv = count.clamp_min(1).float().reciprocal()
     if reduction == "none":
-        return loss, lse2
-    loss = loss.sum()
-    return (loss / count[0].clamp_min(1) if reduction == "mean" else loss), lse2
+        return loss.view(rows.shape), inv
+    return (loss.sum() * inv[0] if reduction == "mean" else loss.sum()), inv
+
+
+def _native_loss(hidden, weight, targets, indices, tau, ignore_index, reduction, vstart, group, max_workspace_mb):
+    nbytes = max_workspace_mb << 20
+    if _world(group) > 1 or getattr(weight, "main_grad", None) is not None:
+        with_grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+        return _HeadLossFn.apply(hidden, weight, targets, indices, tau, ignore_index, reduction, vstart, group, nbytes,
+                                 with_grad)
+    return ext().linear_head_loss(hidden, weight, targets, indices, tau, ignore_index, _REDUCTIONS[reduction], vstart,
+                                  nbytes)
 
 
 def _check(name, hidden, weight, reduction, max_workspace_mb):
@@ -209,9 +189,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     if labels.device != hidden.device:
         raise ValueError(f"linear_cross_entropy: labels on {labels.device}, hidden on {hidden.device}")
     if hidden.is_cuda:
-        with_grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
-        return _HeadLossFn.apply(hidden, weight, labels.reshape(-1).contiguous(), None, None, 1.0, ignore_index,
-                                 reduction, vocab_start, group, max_workspace_mb << 20, with_grad)
+        return _native_loss(hidden, weight, labels.reshape(-1).contiguous(), None, 1.0, ignore_index, reduction,
+                            vocab_start, group, max_workspace_mb)
     lab = labels.reshape(-1)
     valid = lab != ignore_index
     h = torch.where(valid[:, None], hidden.reshape(-1, hidden.shape[-1]), 0.0)
@@ -272,11 +251,10 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_valu
     if hidden.is_cuda:
         if values.dtype not in (torch.float32, torch.bfloat16, torch.float16):
             raise TypeError(f"linear_distillation: teacher values must be fp32, bf16 or fp16, got {values.dtype}")
-        with_grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
         values = values if values.stride(-1) == 1 else values.contiguous()
         indices = indices if indices.stride(-1) == 1 else indices.contiguous()
-        return _HeadLossFn.apply(hidden, weight, None, values, indices, float(temperature), 0, reduction, 0, None,
-                                 max_workspace_mb << 20, with_grad)
+        return _native_loss(hidden, weight, values, indices, float(temperature), 0, reduction, 0, None,
+                            max_workspace_mb)
     there = (indices >= 0) & (indices < weight.shape[0]) & (values != float("-inf"))
     valid = there.any(1)
     h = torch.where(valid[:, None], hidden.reshape(-1, hidden.shape[-1]), 0.0)

@@ -96,8 +96,8 @@ __global__ void __launch_bounds__(256)
 
 // ------------------------------------------------------------------ stable radix sort of (id, token)
 constexpr int kBits = 9, kBins = 1 << kBits;
-constexpr int kSortThreads = 256, kSortItems = 8, kSortTile = kSortThreads * kSortItems;
-constexpr int kSmallThreads = 1024, kSmallMax = 8 * kSmallThreads;
+constexpr int kSortThreads = 256, kSortItems = 4, kSortTile = kSortThreads * kSortItems;
+constexpr int kSmallThreads = 1024, kSmallItems = 2, kSmallMax = kSmallItems * kSmallThreads;
 
 struct SortParams {
   const int64_t* ids;
@@ -150,34 +150,32 @@ __device__ __forceinline__ int bins_before(int mine, int* warp_sums) {
   return before;
 }
 
-// Up to kSmallMax tokens: all passes in one CTA, items in shared memory (8 us at 8192 tokens and two passes, against
-// 25 us of the four launches below).
-__global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortParams p, int bits, int2* __restrict__ out) {
-  extern __shared__ int2 small_items[];  // [n]
-  __shared__ unsigned short count[kSmallThreads / 32][kBins];
+// Up to kSmallMax tokens: all passes in one CTA, items in shared memory.
+__global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortParams p, int bits, int2* out) {
+  __shared__ __align__(16) unsigned short count[kSmallThreads / 32][kBins];
   __shared__ int warp_sums[kSmallThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rounds = (p.n + kSmallThreads - 1) / kSmallThreads, base = warp * 32 * rounds + lane;
   if (p.present != nullptr)
     for (int i = threadIdx.x; i < p.words; i += kSmallThreads) p.present[i] = 0u;
-  int2 item[8];
-  int rank[8], bin[8];
+  int2 item[kSmallItems];
+  int rank[kSmallItems], bin[kSmallItems];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < kSmallItems; ++j) {
     const int i = base + j * 32;
     item[j] = make_int2(0, -1);
     if (j < rounds && i < p.n) item[j] = make_int2(sort_key(p, i), i);
   }
   __syncthreads();  // the bitmap is zeroed
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < kSmallItems; ++j)
     if (item[j].y >= 0) mark_present(p, item[j].x);
   for (int shift = 0; shift < bits; shift += kBits) {
     for (int i = threadIdx.x; i < kSmallThreads / 32 * kBins / 2; i += kSmallThreads)
       reinterpret_cast<unsigned*>(&count[0][0])[i] = 0u;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kSmallItems; ++j) {
       if (j >= rounds) break;
       bin[j] = item[j].y >= 0 ? (item[j].x >> shift) & (kBins - 1) : kBins;
       rank[j] = warp_rank(count[warp], bin[j]);
@@ -198,40 +196,43 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortParams p,
     __syncthreads();
     const bool done = shift + kBits >= bits;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < rounds && bin[j] < kBins) (done ? out : small_items)[count[warp][bin[j]] + rank[j]] = item[j];
+    for (int j = 0; j < kSmallItems; ++j)
+      if (j < rounds && bin[j] < kBins) out[count[warp][bin[j]] + rank[j]] = item[j];
     if (done) return;
-    __syncthreads();
+    __syncthreads();  // through global memory: one CTA wrote it all
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kSmallItems; ++j) {
       const int i = base + j * 32;
-      if (j < rounds && i < p.n) item[j] = small_items[i];
+      if (j < rounds && i < p.n) item[j] = out[i];
     }
   }
 }
 
-// hist[tile][bin] = items of the tile in the bin. The first pass also zeroes the bitmap.
+// First pass: hist[tile][bin] = items of the tile in the bin. Zeroes the bitmap and the later passes' histograms.
 __global__ void __launch_bounds__(kSortThreads)
-    sort_count_kernel(SortParams p, const int2* __restrict__ in, int shift, int* __restrict__ hist) {
+    sort_count_kernel(SortParams p, int* __restrict__ hist, int tiles, int passes) {
   __shared__ int bins[kBins];
   for (int i = threadIdx.x; i < kBins; i += kSortThreads) bins[i] = 0;
-  if (in == nullptr && p.present != nullptr)
-    for (int i = blockIdx.x * kSortThreads + threadIdx.x; i < p.words; i += gridDim.x * kSortThreads) p.present[i] = 0u;
+  const int at = blockIdx.x * kSortThreads + threadIdx.x, all = gridDim.x * kSortThreads;
+  if (p.present != nullptr)
+    for (int i = at; i < p.words; i += all) p.present[i] = 0u;
+  for (int i = tiles * kBins + at; i < passes * tiles * kBins; i += all) hist[i] = 0;
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kSortItems; ++j) {
     const int i = blockIdx.x * kSortTile + j * kSortThreads + threadIdx.x;
-    if (i < p.n) atomicAdd(&bins[(sort_item(p, in, i).x >> shift) & (kBins - 1)], 1);
+    if (i < p.n) atomicAdd(&bins[sort_key(p, i) & (kBins - 1)], 1);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < kBins; i += kSortThreads) hist[blockIdx.x * kBins + i] = bins[i];
 }
 
-// Moves a tile's items to their places, which every CTA works out from the whole histogram. The first pass also
-// marks the bitmap.
+// Moves a tile's items to their places, which every CTA works out from the whole histogram, and counts them for the
+// next pass by the tile that they land in (integer atomics: the counts do not depend on their order). The first pass
+// also marks the bitmap.
 __global__ void __launch_bounds__(kSortThreads)
     sort_move_kernel(SortParams p, const int2* __restrict__ in, int shift, int tiles, const int* __restrict__ hist,
-                     int2* __restrict__ out) {
+                     int* __restrict__ next_hist, int2* __restrict__ out) {
   constexpr int kWarps = kSortThreads / 32;
   __shared__ int count[kWarps][kBins];
   __shared__ int warp_sums[kWarps];
@@ -277,7 +278,12 @@ __global__ void __launch_bounds__(kSortThreads)
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kSortItems; ++j)
-    if (bin[j] < kBins) out[count[warp][bin[j]] + rank[j]] = item[j];
+    if (bin[j] < kBins) {
+      const int to = count[warp][bin[j]] + rank[j];
+      out[to] = item[j];
+      if (next_hist != nullptr)
+        atomicAdd(next_hist + to / kSortTile * kBins + ((item[j].x >> (shift + kBits)) & (kBins - 1)), 1);
+    }
 }
 
 // ------------------------------------------------------------------ sums over runs of equal ids
@@ -334,15 +340,16 @@ __device__ __forceinline__ void write_row(G* dw, float scale, float (&acc)[VEC])
   else RowVec<G, VEC>::store(dw, acc);
 }
 
-// CTAs [0, pieces * slices) sum `piece` sorted tokens each over one slice of the columns; without ADD the CTAs after
-// them zero the rows that no token has.
+// pieces * slices CTAs sum `piece` sorted tokens each over one slice of the columns; without ADD the others, spread
+// evenly among them because they only write, zero the rows that no token has.
 template <typename T, typename G, int VEC, bool ADD>
 __global__ void __launch_bounds__(kSumThreads)
     embed_sum_kernel(SumParams p, const T* __restrict__ dout, G* __restrict__ dw) {
   __shared__ int2 items[kPieceMax + 2];
-  const int block = blockIdx.x;
-  if (block >= p.pieces * p.slices) {
-    const int word = block - p.pieces * p.slices;
+  const unsigned sums = p.pieces * p.slices;
+  const unsigned block = static_cast<unsigned>(static_cast<uint64_t>(blockIdx.x) * sums / gridDim.x);
+  if (static_cast<unsigned>((static_cast<uint64_t>(blockIdx.x) + 1) * sums / gridDim.x) == block) {
+    const int word = blockIdx.x - block;
     const int64_t v0 = static_cast<int64_t>(word) * kZeroRows;
     unsigned empty = ~__ldg(p.present + word);
     if (p.V - v0 < 32) empty &= (1u << (p.V - v0)) - 1u;
@@ -434,33 +441,30 @@ bool vectors_ok(const at::Tensor& t, int64_t H, int vec) {
   return H % vec == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
 }
 
+int sort_passes(int64_t V) {
+  int bits = 1;
+  while (bits < 31 && (V >> bits) != 0) ++bits;  // keys go up to V
+  return (bits + kBits - 1) / kBits;
+}
+
 // Sorts into `a` or `b` ([n] pairs each; b and hist only for more than kSmallMax tokens); returns the sorted one.
 const int2* sort_tokens(const SortParams& p, int2* a, int2* b, int* hist, cudaStream_t stream) {
-  int bits = 1;
-  while (bits < 31 && (p.V >> bits) != 0) ++bits;  // keys go up to V
   if (p.n <= kSmallMax) {
-    static bool attr_set[16] = {false};
-    int dev;
-    NTB_CUDA_CHECK(cudaGetDevice(&dev));
-    if (!attr_set[dev & 15]) {
-      NTB_CUDA_CHECK(cudaFuncSetAttribute(sort_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          kSmallMax * static_cast<int>(sizeof(int2))));
-      attr_set[dev & 15] = true;
-    }
-    const size_t smem = bits > kBits ? p.n * sizeof(int2) : 0;
-    sort_small_kernel<<<1, kSmallThreads, smem, stream>>>(p, bits, a);
+    sort_small_kernel<<<1, kSmallThreads, 0, stream>>>(p, sort_passes(p.V) * kBits, a);
     NTB_LAUNCH_CHECK(1);
     return a;
   }
-  const int tiles = (p.n + kSortTile - 1) / kSortTile;
+  const int tiles = (p.n + kSortTile - 1) / kSortTile, passes = sort_passes(p.V);
+  sort_count_kernel<<<tiles, kSortThreads, 0, stream>>>(p, hist, tiles, passes);
   const int2* in = nullptr;
-  for (int shift = 0; shift < bits; shift += kBits) {
+  for (int i = 0; i < passes; ++i) {
     int2* out = in == a ? b : a;
-    sort_count_kernel<<<tiles, kSortThreads, 0, stream>>>(p, in, shift, hist);
-    sort_move_kernel<<<tiles, kSortThreads, 0, stream>>>(p, in, shift, tiles, hist, out);
-    NTB_LAUNCH_CHECK(2);
+    int* h = hist + static_cast<int64_t>(i) * tiles * kBins;
+    sort_move_kernel<<<tiles, kSortThreads, 0, stream>>>(p, in, i * kBits, tiles, h,
+                                                         i + 1 < passes ? h + tiles * kBins : nullptr, out);
     in = out;
   }
+  NTB_LAUNCH_CHECK(1 + passes);
   return in;
 }
 
@@ -531,7 +535,7 @@ void embed_backward(const at::Tensor& ids, const at::Tensor& dout, double scale,
   const bool small = n <= kSmallMax;
   const int64_t tiles = (n + kSortTile - 1) / kSortTile;
   const int64_t words = add ? 0 : (V + 31) / 32;
-  const int64_t part_n = p.pieces > 1 ? (2 * p.pieces * H + 3) / 4 * 4 : 0, hist_n = small ? 0 : kBins * tiles;
+  const int64_t part_n = p.pieces > 1 ? (2 * p.pieces * H + 3) / 4 * 4 : 0, hist_n = small ? 0 : kBins * tiles * sort_passes(V);
   auto ws = at::empty({part_n + (small ? 2 : 4) * n + hist_n + words}, dout.options().dtype(at::kFloat));
   float* at_ws = ws.data_ptr<float>();
   p.part = at_ws;

@@ -255,7 +255,7 @@ struct GatherParams {
   int tokens; // per CTA
 };
 
-constexpr int kGatherThreads = 256;
+constexpr int kGatherThreads = 256, kGatherAhead = 4;
 
 __device__ __forceinline__ void zero_row(bf16* dst, int H) {
   for (int i = threadIdx.x & 31; i < H / 8; i += 32) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
@@ -269,6 +269,7 @@ __device__ __forceinline__ void zero_row(bf16* dst, int H) {
 template <bool KNOWN>
 __global__ void __launch_bounds__(kGatherThreads) head_gather_kernel(GatherParams p) {
   __shared__ int red[2][kGatherThreads / 32];
+  __shared__ float dots[kGatherThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = blockIdx.x * p.tokens, t1 = min(p.T, t0 + p.tokens);
   auto live = [&](int t) { return p.labels != nullptr ? p.labels[t] != p.ignore_index : p.st.live[t] != 0; };
@@ -301,8 +302,11 @@ __global__ void __launch_bounds__(kGatherThreads) head_gather_kernel(GatherParam
       p.st.head->inv = p.mean ? 1.f / static_cast<float>(max(count, 1)) : 1.f;
     }
   }
+  // Every warp walks all of the CTA's tokens to know their places (32 at a time) and copies its share: whole rows,
+  // or with one token a CTA its part of the row.
   const int vecs = p.H / 8;
-  // Every warp walks all of the CTA's tokens to know their places (32 at a time) and copies its share.
+  const bool alone = p.tokens == 1;
+  const int first = alone ? static_cast<int>(threadIdx.x) : lane, step = alone ? kGatherThreads : 32;
   for (int b = t0; b < t1; b += 32) {
     const int mine = b + lane;
     int place = -1;
@@ -319,7 +323,7 @@ __global__ void __launch_bounds__(kGatherThreads) head_gather_kernel(GatherParam
         else p.st.loss[mine] = 0.f;
       }
     }
-    for (int i = warp; i < 32 && b + i < t1; i += kGatherThreads / 32) {
+    for (int i = alone ? 0 : warp; i < 32 && b + i < t1; i += kGatherThreads / 32) {
       const int t = b + i, row = __shfl_sync(0xffffffffu, place, i);
       int target = kIgnored;
       if (!KNOWN && p.labels != nullptr) {
@@ -333,28 +337,45 @@ __global__ void __launch_bounds__(kGatherThreads) head_gather_kernel(GatherParam
       }
       const uint4* src = reinterpret_cast<const uint4*>(p.h + t * p.ldh);
       uint4* dst = reinterpret_cast<uint4*>(p.x + static_cast<long>(row) * p.H);
-      if (target >= 0 && target != kNowhere) {
-        const uint4* wr = reinterpret_cast<const uint4*>(p.w + target * p.ldw);
-        float dot[2] = {0.f, 0.f};
-#pragma unroll 4
-        for (int k = lane; k < vecs; k += 32) {
-          const uint4 a = __ldg(src + k), c = __ldg(wr + k);
-          dst[k] = a;
-          dot[0] = fmaf(bf16_lo(a.x), bf16_lo(c.x), dot[0]);
-          dot[1] = fmaf(bf16_hi(a.x), bf16_hi(c.x), dot[1]);
-          dot[0] = fmaf(bf16_lo(a.y), bf16_lo(c.y), dot[0]);
-          dot[1] = fmaf(bf16_hi(a.y), bf16_hi(c.y), dot[1]);
-          dot[0] = fmaf(bf16_lo(a.z), bf16_lo(c.z), dot[0]);
-          dot[1] = fmaf(bf16_hi(a.z), bf16_hi(c.z), dot[1]);
-          dot[0] = fmaf(bf16_lo(a.w), bf16_lo(c.w), dot[0]);
-          dot[1] = fmaf(bf16_hi(a.w), bf16_hi(c.w), dot[1]);
+      const bool dotted = target >= 0 && target != kNowhere;
+      const uint4* wr = reinterpret_cast<const uint4*>(p.w + (dotted ? target : 0) * p.ldw);
+      float dot[2] = {0.f, 0.f};
+      for (int k0 = first; k0 < vecs; k0 += step * kGatherAhead) {
+        uint4 a[kGatherAhead], c[kGatherAhead];
+#pragma unroll
+        for (int u = 0; u < kGatherAhead; ++u) {
+          const int k = k0 + u * step;
+          if (k < vecs) {
+            a[u] = __ldg(src + k);
+            if (dotted) c[u] = __ldg(wr + k);
+          }
         }
-        const float sum = warp_sum(dot[0] + dot[1]);
-        if (lane == 0) p.st.exact[row] = sum * p.scale2;
-      } else {
-#pragma unroll 4
-        for (int k = lane; k < vecs; k += 32) dst[k] = __ldg(src + k);
+#pragma unroll
+        for (int u = 0; u < kGatherAhead; ++u) {
+          const int k = k0 + u * step;
+          if (k >= vecs) break;
+          dst[k] = a[u];
+          if (!dotted) continue;
+          dot[0] = fmaf(bf16_lo(a[u].x), bf16_lo(c[u].x), dot[0]);
+          dot[1] = fmaf(bf16_hi(a[u].x), bf16_hi(c[u].x), dot[1]);
+          dot[0] = fmaf(bf16_lo(a[u].y), bf16_lo(c[u].y), dot[0]);
+          dot[1] = fmaf(bf16_hi(a[u].y), bf16_hi(c[u].y), dot[1]);
+          dot[0] = fmaf(bf16_lo(a[u].z), bf16_lo(c[u].z), dot[0]);
+          dot[1] = fmaf(bf16_hi(a[u].z), bf16_hi(c[u].z), dot[1]);
+          dot[0] = fmaf(bf16_lo(a[u].w), bf16_lo(c[u].w), dot[0]);
+          dot[1] = fmaf(bf16_hi(a[u].w), bf16_hi(c[u].w), dot[1]);
+        }
       }
+      if (!dotted) continue;
+      float sum = warp_sum(dot[0] + dot[1]);
+      if (alone) {
+        if (lane == 0) dots[warp] = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < kGatherThreads / 32; ++u) sum += dots[u];
+      }
+      if (lane == 0 && (!alone || warp == 0)) p.st.exact[row] = sum * p.scale2;
     }
   }
   for (int r = count + blockIdx.x * (kGatherThreads / 32) + warp; r < max(64, (count + 63) & ~63);
@@ -466,7 +487,7 @@ struct RowParams {
   float* out;
 };
 
-constexpr int kRowThreads = 512;
+constexpr int kRowThreads = 256, kRowAhead = 4;
 
 // Joins (maximum, sum) pairs over the block; every thread returns log2 of the whole sum.
 __device__ __forceinline__ float row_join(float2 a, float2* red) {
@@ -517,6 +538,15 @@ __global__ void __launch_bounds__(kRowThreads) head_row_kernel(RowParams p) {
   if (row < live) {
     const int token = p.map[row];
     const float2* part = p.part + static_cast<long>(row) * p.n_tiles;
+    // G's first vectors are requested before the statistics are joined.
+    uint4* g = WRITE ? reinterpret_cast<uint4*>(p.codes + row * p.ldg) : nullptr;
+    const int vecs = (p.V + 7) / 8;
+    uint4 ahead[kRowAhead];
+    if constexpr (WRITE) {
+#pragma unroll
+      for (int u = 0; u < kRowAhead; ++u)
+        if (threadIdx.x + u * kRowThreads < vecs) ahead[u] = g[threadIdx.x + u * kRowThreads];
+    }
     float2 a = make_float2(-INFINITY, 0.f);
     for (int i = threadIdx.x; i < p.n_tiles; i += kRowThreads) {
       const float2 b = part[i];
@@ -535,17 +565,26 @@ __global__ void __launch_bounds__(kRowThreads) head_row_kernel(RowParams p) {
       lse2 += log1pf(ex2(only - lse2) - ex2(picked[0] - lse2)) * (1.f / kLn2);
     }
     if constexpr (WRITE) {
-      uint4* g = reinterpret_cast<uint4*>(p.codes + row * p.ldg);
-      const int vecs = (p.V + 7) / 8;
-#pragma unroll 4
-      for (int i = threadIdx.x; i < vecs; i += kRowThreads) {
-        const uint4 c = g[i];
-        const float base = row_smem[i >> p.tile_shift] - lse2;
-        const uint32_t in[4] = {c.x, c.y, c.z, c.w};
-        uint32_t out[4];
+      for (int i0 = threadIdx.x; i0 < vecs; i0 += kRowThreads * kRowAhead) {
+        uint4 now[kRowAhead];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) out[j] = pack_bf16x2(code_prob(in[j] & 0xffffu, base), code_prob(in[j] >> 16, base));
-        g[i] = make_uint4(out[0], out[1], out[2], out[3]);
+        for (int u = 0; u < kRowAhead; ++u) {
+          now[u] = ahead[u];
+          const int i = i0 + (kRowAhead + u) * kRowThreads;
+          if (i < vecs) ahead[u] = g[i];
+        }
+#pragma unroll
+        for (int u = 0; u < kRowAhead; ++u) {
+          const int i = i0 + u * kRowThreads;
+          if (i >= vecs) break;
+          const float base = row_smem[i >> p.tile_shift] - lse2;
+          const uint32_t in[4] = {now[u].x, now[u].y, now[u].z, now[u].w};
+          uint32_t out[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            out[j] = pack_bf16x2(code_prob(in[j] & 0xffffu, base), code_prob(in[j] >> 16, base));
+          g[i] = make_uint4(out[0], out[1], out[2], out[3]);
+        }
       }
     }
     __syncthreads();  // all have read `picked`, and G's pass is done
@@ -818,8 +857,8 @@ at::Tensor gather(const Head& hd, const State& st, const int64_t* labels, int64_
   p.st.loss = loss;
   p.x = reinterpret_cast<bf16*>(x.data_ptr());
   p.dh = dh;
-  // 16 tokens a CTA; more from 65536 on, so that the counting reads T labels at most 4096 times.
-  p.tokens = static_cast<int>(std::max<int64_t>(16, round_up((hd.T + 4095) / 4096, 32)));
+  // One token a CTA up to 2048, 16 then; more from 65536 on, so that the labels are read at most 4096 times.
+  p.tokens = hd.T <= 2048 ? 1 : static_cast<int>(std::max<int64_t>(16, round_up((hd.T + 4095) / 4096, 32)));
   const unsigned blocks = static_cast<unsigned>((hd.T + p.tokens - 1) / p.tokens);
   if (known) head_gather_kernel<true><<<blocks, kGatherThreads, 0, hd.stream>>>(p);
   else head_gather_kernel<false><<<blocks, kGatherThreads, 0, hd.stream>>>(p);

@@ -108,8 +108,7 @@ static TileChoice pick_tiles(int64_t M, int64_t N, int64_t K, int nsm, bool can_
 //   out: [M,N] bf16 or fp32 with unit inner stride
 static void gemm_bf16_impl(const at::Tensor& a, const at::Tensor& b, at::Tensor& out,
                            const c10::optional<at::Tensor>& bias, bool a_mn, bool b_mn, bool accumulate, double alpha,
-                           const std::vector<int64_t>& pub_flags, int64_t pub_epoch, unsigned int* pub_ctr,
-                           const GemmTokenRows* tok = nullptr) {
+                           const std::vector<int64_t>& pub_flags, int64_t pub_epoch, unsigned int* pub_ctr) {
   TORCH_CHECK(a.is_cuda() && b.is_cuda() && out.is_cuda(), "gemm_bf16: CUDA tensors required");
   TORCH_CHECK(a.scalar_type() == at::kBFloat16 && b.scalar_type() == at::kBFloat16, "gemm_bf16: bf16 operands");
   TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && out.dim() == 2, "gemm_bf16: 2-D tensors");
@@ -148,19 +147,8 @@ static void gemm_bf16_impl(const at::Tensor& a, const at::Tensor& b, at::Tensor&
   p.groups = 1;
   p.b_group_rows = 0;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream(a.get_device());
-  TileChoice tc = pick_tiles(M, N, K, num_sms(a.get_device()),
-                             accumulate && p.c_f32 && !bias.has_value() && tok == nullptr);
-  if (tok != nullptr) {
-    p.rows = tok->rows;
-    p.rows_base = tok->rows_base;
-    p.rows_are_k = tok->rows_are_k ? 1 : 0;
-    p.slice_stride = tok->slice_stride;
-    p.alpha_dev = tok->alpha_dev;
-    if (tok->splits > 1) {
-      TORCH_CHECK(p.c_f32 && !accumulate && tok->slice_stride >= M * p.ldc, "gemm_bf16: slices need their own fp32 rows");
-      tc = {N > 128, tok->splits};
-    }
-  }
+  const TileChoice tc = pick_tiles(M, N, K, num_sms(a.get_device()),
+                                   accumulate && p.c_f32 && !bias.has_value());
   const bool wide = tc.wide;
   p.splits = tc.splits;
   if (!pub_flags.empty()) {
@@ -206,11 +194,6 @@ static void gemm_bf16_impl(const at::Tensor& a, const at::Tensor& b, at::Tensor&
     NTB_GEMM_CASE(128, true, true)
   }
 #undef NTB_GEMM_CASE
-}
-
-void gemm_bf16_tokens(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool a_mn, bool b_mn, bool accumulate,
-                      const GemmTokenRows& tok) {
-  gemm_bf16_impl(a, b, out, c10::nullopt, a_mn, b_mn, accumulate, tok.alpha, {}, 0, nullptr, &tok);
 }
 
 void gemm_bf16(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, const c10::optional<at::Tensor>& bias,

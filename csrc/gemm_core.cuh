@@ -33,9 +33,6 @@ struct GemmParams {
   // (tile, slice) unit adds its partial product into C with vector atomics, so the sum's
   // rounding order varies from run to run (fp32 low bits only).
   int splits;
-  // With splits > 1 and slice_stride > 0 (elements, fp32 C, no accumulate): slice s writes its partial product to
-  // C + s * slice_stride with plain stores instead, for a later pass that adds the slices in a fixed order.
-  long slice_stride;
   // Rows known only on the device (plain GEMM, optional): when `rows` is set, the token extent is
   // clamp(*rows - rows_base, 0, its host value) instead of its host value - the M extent, or K when rows_are_k
   // (a sum over tokens; the operands' rows up to the next multiple of 64 are then zeros). A launch without rows
@@ -43,7 +40,7 @@ struct GemmParams {
   const int* rows;
   int rows_base;
   int rows_are_k;
-  const float* alpha_dev;  // device factor of alpha (optional)
+  const float* alpha_dev;  // device factor of alpha (gemm_wide.cu)
   // Publication (plain GEMM, optional): when pub_n > 0, the last CTA to finish makes the whole C
   // visible system-wide (fence.sc.sys) and stores pub_epoch into pub_flag[0..pub_n) - the epoch
   // words of the peers that read C over NVLink. pub_ctr: a device u32 that is zero at rest.
@@ -107,13 +104,11 @@ __device__ __forceinline__ void tile_coords(int tile, int num_m, int num_n, int&
 // final rounding. m0: first row of the warp; n0: first column of the tile.
 template <int BN>
 __device__ __forceinline__ void epilogue_tile(uint32_t t_row, float* stage, const GemmParams& p, long m0, int n0,
-                                              bool vec_ok, long m_end, bool red = false,
-                                              long c_off = 0) {
+                                              bool vec_ok, long m_end, bool red = false) {
   const int lane = threadIdx.x & 31;
   const bool f32 = p.c_f32 != 0;
   // red: a K-slice of a split GEMM (fp32 C) - the partial is added with atomics, C is not read.
   const bool acc = p.accumulate != 0 && !red;
-  const float alpha = p.alpha_dev != nullptr ? p.alpha * __ldg(p.alpha_dev) : p.alpha;
 #pragma unroll 1
   for (int g = 0; g < BN; g += 64) {
     const int cg = n0 + g;
@@ -153,7 +148,7 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, float* stage, cons
       for (int u = 0; u < 4; ++u) {
         const int c = j * 4 + u;
         const uint32_t bits = c < 32 ? r0[c] : r1[c - 32];
-        float x = __uint_as_float(bits) * alpha;
+        float x = __uint_as_float(bits) * p.alpha;
         if (p.bias != nullptr && !red && cg + c < p.N) x += __bfloat162float(p.bias[cg + c]);
         w[u] = x;
       }
@@ -161,7 +156,7 @@ __device__ __forceinline__ void epilogue_tile(uint32_t t_row, float* stage, cons
     }
     __syncwarp();
     if (f32) {
-      float* C = reinterpret_cast<float*>(p.C) + c_off;
+      float* C = reinterpret_cast<float*>(p.C);
 #pragma unroll
       for (int it = 0; it < 16; ++it) {
         const int row = it * 2 + (lane >> 4), ch = lane & 15;
@@ -279,10 +274,8 @@ struct StoreEpilogue {
   __device__ __forceinline__ void begin(const Params&, long, int) {}
   template <int BN>
   __device__ __forceinline__ void tile(uint32_t t_row, float* stage, const Params& p, long m0, int n0, bool vec_ok,
-                                       long m_end, int slice, int) {
-    const bool split = p.splits > 1;
-    epilogue_tile<BN>(t_row, stage, p, m0, n0, vec_ok, m_end, split && p.slice_stride == 0,
-                      split ? slice * p.slice_stride : 0);
+                                       long m_end, int) {
+    epilogue_tile<BN>(t_row, stage, p, m0, n0, vec_ok, m_end, p.splits > 1);
   }
 };
 
@@ -448,11 +441,11 @@ __global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
       const TileInfo ti = tile_info<GM>(p, tile, num_m, num_n, num_kb, BM, BK);
       const long m0 = static_cast<long>(ti.mb) * BM + q * 32;
       if constexpr (GM != 2) epi.begin(p, m0, ti.nb * BN + epart * (BN / 2));
-      if (!mbar_wait(&tfull[acc], acc_phase, p.status, kStatusTimeoutEpilogue)) break;
+      if (!mbar_wait_warp(&tfull[acc], acc_phase, p.status, kStatusTimeoutEpilogue)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
       if constexpr (GM != 2) {
-        epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, ti.slice, epart);
+        epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, epart);
       } else if (ti.nkb > 0) {
         // Expert block: rows [group * M, group * M + M) of the stacked output; an expert without
         // rows contributes nothing (its accumulator was never written).
@@ -565,100 +558,106 @@ __global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
   const uint32_t full0 = cluster_addr(full, 0);      // CTA 0's full[s] at full0 + 8 s
   const uint32_t tempty0 = cluster_addr(tempty, 0);  // CTA 0's tempty[b] at tempty0 + 8 b
 
+  // The producer's and the issuer's loops are run by whole warps, with one elected lane for the asynchronous
+  // instructions: loop variables and descriptors are then warp-uniform and live in uniform registers. Run by a single
+  // lane, the issuer took about 600 clocks for the 512 clocks of tensor work of a K block.
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t filled_mask = 0;
-      uint32_t last_phase[STAGES];
-#pragma unroll
-      for (int s = 0; s < STAGES; ++s) last_phase[s] = 0;
-      bool ok = true;
-      for (int tile = pair; tile < num_tiles && ok; tile += npairs) {
-        const TileInfo ti = tile_info<0>(p, tile, num_m, num_n, num_kb, 2 * BM, BK);
-        const int arow = ti.mb * 2 * BM + static_cast<int>(rank) * BM;
-        const int bcol = ti.nb * BN + static_cast<int>(rank) * (BN / 2);
-        for (int kq = 0; kq < ti.nkb; ++kq) {
-          const int kb = ti.kb0 + kq;
-          if (!mbar_wait(&empty[stage], phase ^ 1, p.status, kStatusTimeoutProducer)) {
-            ok = false;
-            break;
-          }
+    const bool leader = elect_one();
+    uint32_t stage = 0, phase = 0, filled = 0, last = 0;  // bit s: stage s was filled, in that phase
+    bool ok = true;
+    for (int tile = pair; tile < num_tiles && ok; tile += npairs) {
+      const TileInfo ti = tile_info<0>(p, tile, num_m, num_n, num_kb, 2 * BM, BK);
+      const int arow = ti.mb * 2 * BM + static_cast<int>(rank) * BM;
+      const int bcol = ti.nb * BN + static_cast<int>(rank) * (BN / 2);
+      int k0 = ti.kb0 * BK;
+      for (int kq = 0; kq < ti.nkb; ++kq, k0 += BK) {
+        if (!mbar_wait_warp(&empty[stage], phase ^ 1, p.status, kStatusTimeoutProducer)) {
+          ok = false;
+          break;
+        }
+        if (leader) {
           // CTA 0 expects the bytes of both CTAs' loads on its barrier.
           if (rank == 0) mbar_expect_tx(&full[stage], 2 * (A_BYTES + B_BYTES));
-          const uint32_t bar = full0 + 8u * static_cast<uint32_t>(stage);
+          const uint32_t bar = full0 + 8u * stage;
           uint8_t* a_dst = sA + stage * A_BYTES;
           uint8_t* b_dst = sB + stage * B_BYTES;
           if constexpr (!A_MN) {
-            tma_load_2d_pair(a_dst, &tmA, bar, kb * BK, arow);
+            tma_load_2d_pair(a_dst, &tmA, bar, k0, arow);
           } else {
 #pragma unroll
-            for (int j = 0; j < BM / 64; ++j) tma_load_2d_pair(a_dst + j * 8192, &tmA, bar, arow + j * 64, kb * BK);
+            for (int j = 0; j < BM / 64; ++j) tma_load_2d_pair(a_dst + j * 8192, &tmA, bar, arow + j * 64, k0);
           }
           if constexpr (!B_MN) {
-            tma_load_2d_pair(b_dst, &tmB, bar, kb * BK, bcol);
+            tma_load_2d_pair(b_dst, &tmB, bar, k0, bcol);
           } else {
 #pragma unroll
-            for (int j = 0; j < (BN / 2) / 64; ++j)
-              tma_load_2d_pair(b_dst + j * 8192, &tmB, bar, bcol + j * 64, kb * BK);
-          }
-          filled_mask |= 1u << stage;
-          last_phase[stage] = phase;
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
+            for (int j = 0; j < (BN / 2) / 64; ++j) tma_load_2d_pair(b_dst + j * 8192, &tmB, bar, bcol + j * 64, k0);
           }
         }
+        __syncwarp();
+        filled |= 1u << stage;
+        last = (last & ~(1u << stage)) | (phase << stage);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
-      // CTA 0's barriers count both CTAs' bytes: never leave with a TMA write still landing.
-      if (rank == 0)
-        for (int s = 0; s < STAGES; ++s)
-          if (filled_mask & (1u << s)) mbar_wait(&full[s], last_phase[s], nullptr, 0) || true;
     }
+    // CTA 0's barriers count both CTAs' bytes: never leave with a TMA write still landing.
+    if (rank == 0)
+      for (int s = 0; s < STAGES; ++s)
+        if (filled >> s & 1u) mbar_wait(&full[s], last >> s & 1u, nullptr, 0);
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int acc = 0;
-      uint32_t acc_phase = 0;
+    if (rank == 0) {
+      // K-major: 16 elements (32 B) further inside the 128 B swizzle row; MN-major: 16 K rows of 128 B.
+      constexpr uint32_t A_K = (A_MN ? 2048 : 32) >> 4, B_K = (B_MN ? 2048 : 32) >> 4;
+      const bool leader = elect_one();
+      const uint64_t a0 = make_smem_desc_sw128(smem_u32(sA), A_MN ? 8192 : 16, 1024);
+      const uint64_t b0 = make_smem_desc_sw128(smem_u32(sB), B_MN ? 8192 : 16, 1024);
+      const uint32_t empty0 = cluster_addr(empty, 0), empty1 = cluster_addr(empty, 1);
+      const uint32_t tfull0 = cluster_addr(tfull, 0), tfull1 = cluster_addr(tfull, 1);
+      const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
       for (int tile = pair; tile < num_tiles && ok; tile += npairs) {
         const int tile_nkb = p.splits > 1 ? tile_info<0>(p, tile, num_m, num_n, num_kb, 2 * BM, BK).nkb : num_kb;
-        if (!mbar_wait(&tempty[acc], acc_phase ^ 1, p.status, kStatusTimeoutMma)) break;
+        if (!mbar_wait_warp(&tempty[acc], acc_phase ^ 1, p.status, kStatusTimeoutMma)) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
+        const uint32_t d_tmem = tmem + acc * BN;
         for (int kb = 0; kb < tile_nkb; ++kb) {
-          if (!mbar_wait(&full[stage], phase, p.status, kStatusTimeoutMma)) {
+          if (!mbar_wait_warp(&full[stage], phase, p.status, kStatusTimeoutMma)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a_base = smem_u32(sA + stage * A_BYTES);
-          const uint32_t b_base = smem_u32(sB + stage * B_BYTES);
+          const uint64_t a = a0 + stage * static_cast<uint32_t>(A_BYTES >> 4);
+          const uint64_t b = b0 + stage * static_cast<uint32_t>(B_BYTES >> 4);
+          if (leader) {
+            umma_f16_ss_pair(d_tmem, a, b, IDESC, kb != 0 ? 1u : 0u);
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            const uint64_t adesc = A_MN ? make_smem_desc_sw128(a_base + k * 2048, 8192, 1024)
-                                        : make_smem_desc_sw128(a_base + k * 32, 16, 1024);
-            const uint64_t bdesc = B_MN ? make_smem_desc_sw128(b_base + k * 2048, 8192, 1024)
-                                        : make_smem_desc_sw128(b_base + k * 32, 16, 1024);
-            umma_f16_ss_pair(d_tmem, adesc, bdesc, IDESC, (kb | k) != 0 ? 1u : 0u);
+            for (int k = 1; k < BK / 16; ++k) umma_f16_ss_pair(d_tmem, a + k * A_K, b + k * B_K, IDESC, 1u);
+            umma_commit_pair(empty0 + 8u * stage);
+            umma_commit_pair(empty1 + 8u * stage);
           }
-          umma_commit_pair(cluster_addr(&empty[stage], 0));
-          umma_commit_pair(cluster_addr(&empty[stage], 1));
+          __syncwarp();
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
           }
         }
         if (!ok) break;
-        umma_commit_pair(cluster_addr(&tfull[acc], 0));
-        umma_commit_pair(cluster_addr(&tfull[acc], 1));
+        if (leader) {
+          umma_commit_pair(tfull0 + 8u * acc);
+          umma_commit_pair(tfull1 + 8u * acc);
+        }
+        __syncwarp();
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
       // Every MMA (which reads both CTAs' shared memory) retires before either CTA moves on.
       if (pair < num_tiles) {
-        umma_commit_pair(cluster_addr(drain, 0));
+        if (leader) umma_commit_pair(cluster_addr(drain, 0));
+        __syncwarp();
         mbar_wait(drain, 0, nullptr, 0);
       }
     }
@@ -674,10 +673,10 @@ __global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
       const TileInfo ti = tile_info<0>(p, tile, num_m, num_n, num_kb, 2 * BM, BK);
       const long m0 = static_cast<long>(ti.mb) * 2 * BM + rank * BM + q * 32;
       epi.begin(p, m0, ti.nb * BN + epart * (BN / 2));
-      if (!mbar_wait(&tfull[acc], acc_phase, p.status, kStatusTimeoutEpilogue)) break;
+      if (!mbar_wait_warp(&tfull[acc], acc_phase, p.status, kStatusTimeoutEpilogue)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
-      epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, ti.slice, epart);
+      epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, epart);
       tc_fence_before();
       mbar_arrive_cluster(tempty0 + 8u * static_cast<uint32_t>(acc));
       acc ^= 1;

@@ -61,18 +61,15 @@ void make_tma_4d_bf16(CUtensorMap* out, const void* base, const int64_t (&dims)[
 void make_tma_2d(CUtensorMap* out, void* base, CUtensorMapDataType dtype, int elem_bytes, int64_t d0, int64_t d1,
                  int64_t ld, int box0, int box1, CUtensorMapSwizzle swz);
 
-// A bf16 GEMM whose token extent is read on the device (gemm.cu; the fields are GemmParams'). With splits > 1 the
-// fp32 result comes as that many partial products, `slice_stride` elements apart.
+// A bf16 GEMM whose token extent is read on the device (gemm_wide.cu; the fields are GemmParams').
 struct GemmTokenRows {
   const int* rows = nullptr;
   int rows_base = 0;
   bool rows_are_k = false;
-  int splits = 1;
-  int64_t slice_stride = 0;
   double alpha = 1.0;
   const float* alpha_dev = nullptr;  // device factor of alpha
 };
-void gemm_bf16_tokens(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool a_mn, bool b_mn, bool accumulate,
-                      const GemmTokenRows& tok);
+void gemm_bf16_wide(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool a_mn, bool accumulate,
+                    const int* map, const GemmTokenRows& tok);
 
 }  // namespace ntb

@@ -18,8 +18,7 @@
 //      3.4e-4 of each probability (bf16 probabilities would have 3.9e-3), 64 powers of two deep;
 //   2. a row kernel that joins the tiles' statistics into lse, computes the row's loss and turns the distances in
 //      place into bf16 p - q, the targets' entries from their fp32 logits;
-//   3. dH = G W, K (the vocabulary) cut into slices whose fp32 partials are added in a fixed order;
-//   4. dW (+)= G^T H.
+//   3. dH = G W and 4. dW (+)= G^T H (gemm_wide.cu), dH's rows going straight to their tokens.
 // That is 6 T V H operations, the least there is, at the price of a chunk of 16-bit G in memory. Where the
 // upstream gradient of each row is only known in the backward pass (per-token losses, a vocabulary sharded over
 // ranks), step 1 runs there a second time with lse known and writes G at once.
@@ -136,7 +135,7 @@ struct HeadEpilogue {
 
   template <int BN>
   __device__ __forceinline__ void tile(uint32_t t_row, float* stage_f, const Params& p, long m0, int n0, bool,
-                                       long m_end, int, int part) {
+                                       long m_end, int part) {
     constexpr int COLS = BN / 2, GROUPS = COLS / 32;
     uint8_t* stage = reinterpret_cast<uint8_t*>(stage_f);
     const int lane = threadIdx.x & 31;
@@ -332,7 +331,7 @@ __global__ void __launch_bounds__(kGatherThreads) head_gather_kernel(GatherParam
         if (lane == 0) p.st.targets[t] = target;
       }
       if (row < 0) {
-        if (!KNOWN && p.dh != nullptr) zero_row(p.dh + static_cast<long>(t) * p.H, p.H);
+        if (p.dh != nullptr) zero_row(p.dh + static_cast<long>(t) * p.H, p.H);
         continue;
       }
       const uint4* src = reinterpret_cast<const uint4*>(p.h + t * p.ldh);
@@ -648,36 +647,6 @@ __global__ void head_fix_kernel(RowParams p, const float* __restrict__ row_scale
   }
 }
 
-// Adds dH's K slices in order, scales the sum by alpha (* *alpha_dev) and puts the compact rows back to their
-// tokens. The rows of tokens without a target were zeroed by the gather, or here with zero_others.
-__global__ void head_dh_kernel(const float* __restrict__ part, int slices, long slice_stride, int H, float alpha,
-                               const float* __restrict__ alpha_dev, const int* __restrict__ place, int row_base,
-                               int row_end, int zero_others, bf16* __restrict__ dh) {
-  const long t = blockIdx.x;
-  const int r = place[t];
-  uint2* out = reinterpret_cast<uint2*>(dh + t * H);
-  if (r < 0) {
-    if (zero_others)
-      for (int i = threadIdx.x; i < H / 4; i += blockDim.x) out[i] = make_uint2(0, 0);
-    return;
-  }
-  if (r < row_base || r >= row_end) return;
-  if (alpha_dev != nullptr) alpha *= *alpha_dev;
-  const float* src = part + static_cast<long>(r - row_base) * H;
-  for (int i = threadIdx.x; i < H / 4; i += blockDim.x) {
-    float4 a = *reinterpret_cast<const float4*>(src + i * 4);
-#pragma unroll 4
-    for (int s = 1; s < slices; ++s) {
-      const float4 b = *reinterpret_cast<const float4*>(src + s * slice_stride + i * 4);
-      a.x += b.x;
-      a.y += b.y;
-      a.z += b.z;
-      a.w += b.w;
-    }
-    out[i] = make_uint2(pack_bf16x2(a.x * alpha, a.y * alpha), pack_bf16x2(a.z * alpha, a.w * alpha));
-  }
-}
-
 // Two bf16 buffers (either may be empty) times *factor, in place; nothing is read or written when the factor is 1
 // (a loss that is itself the root of the backward pass).
 __global__ void __launch_bounds__(256)
@@ -753,31 +722,6 @@ void launch_logits(const at::Tensor& x, const at::Tensor& w, HeadParams p, cudaS
   }
 }
 
-// Slices of the vocabulary for dH. Its 256 x 256 pair tiles (128 x 256 below 256 rows) rarely fill the SMs a whole
-// number of times, by how much only the device knows (the live tokens), and few tokens leave most SMs idle. Modelled
-// time: (waves + half a wave that the last one wastes on average) x (K blocks x 0.30 us + 4 us a unit), plus writing
-// and reading back the fp32 partials.
-int pick_slices(int64_t rows, int64_t H, int64_t V, int nsm) {
-  const bool pair = rows >= 256;
-  const int64_t units = (pair ? (rows + 255) / 256 : (rows + 127) / 128) * ((H + 255) / 256);
-  const double slots = pair ? nsm / 2 : nsm;
-  const int64_t kb = (V + 63) / 64;
-  double best = 1e30;
-  int pick = 1;
-  for (int64_t s = 1; s <= 148; ++s) {
-    const int64_t per = (kb + s - 1) / s;
-    if (s > 1 && (per < 4 || (kb + per - 1) / per != s)) continue;  // no empty slice
-    if (s > 1 && pair && per < 32) break;                           // 2048 of K, where pairs pay
-    const double waves = std::max(1.0, units * s / slots + 0.5);
-    const double us = waves * (per * 0.30 + 4.0) + s * rows * H * 8.0 / 6.0e6;
-    if (us < best * 0.99) {
-      best = us;
-      pick = static_cast<int>(s);
-    }
-  }
-  return pick;
-}
-
 struct Head {
   at::Tensor h, w;  // [T, H], [V, H]
   int64_t T, H, V;
@@ -836,7 +780,7 @@ struct State {
   }
 };
 
-// Gathers the live tokens. dh: rows of the others are zeroed (first pass only).
+// Gathers the live tokens. dh: rows of the others are zeroed.
 at::Tensor gather(const Head& hd, const State& st, const int64_t* labels, int64_t vstart, int64_t ignore_index,
                   bool mean, float* loss, float scale2, bf16* dh, bool known) {
   auto x = at::empty({round_up(hd.T, 64), hd.H}, hd.h.options());
@@ -869,30 +813,20 @@ at::Tensor gather(const Head& hd, const State& st, const int64_t* labels, int64_
 // Gradients of a chunk from its G: dH rows into `dh`, dW into `dw` (overwritten by the first chunk, then added to),
 // both times alpha (* *alpha_dev).
 void chunk_grads(const Head& hd, const at::Tensor& x, const at::Tensor& g, const State& st, int64_t c0, int64_t rows,
-                 double alpha, const float* alpha_dev, at::Tensor* dh, at::Tensor* dw, bool first, bool zero_others) {
+                 double alpha, const float* alpha_dev, at::Tensor* dh, at::Tensor* dw) {
   GemmTokenRows tok;
   tok.rows = &st.v.head->count;
   tok.rows_base = static_cast<int>(c0);
+  tok.alpha = alpha;
+  tok.alpha_dev = alpha_dev;
   auto gv = g.narrow(0, 0, rows).narrow(1, 0, hd.V);
   if (dh) {
-    tok.splits = pick_slices(rows, hd.H, hd.V, num_sms(hd.dev));
-    tok.slice_stride = rows * hd.H;
-    auto part = at::empty({tok.splits * rows, hd.H}, hd.h.options().dtype(at::kFloat));
-    auto out = part.narrow(0, 0, rows);
-    gemm_bf16_tokens(gv, hd.w, out, false, true, false, tok);
-    head_dh_kernel<<<static_cast<unsigned>(hd.T), hd.H >= 512 ? 256 : 64, 0, hd.stream>>>(
-        part.data_ptr<float>(), tok.splits, static_cast<long>(tok.slice_stride), static_cast<int>(hd.H),
-        static_cast<float>(alpha), alpha_dev, st.v.place, static_cast<int>(c0), static_cast<int>(c0 + rows),
-        first && zero_others ? 1 : 0, reinterpret_cast<bf16*>(dh->data_ptr()));
-    NTB_LAUNCH_CHECK(1);
+    auto out = dh->view({hd.T, hd.H});
+    gemm_bf16_wide(gv, hd.w, out, false, false, st.v.map + c0, tok);
   }
   if (dw) {
-    tok.splits = 1;
-    tok.slice_stride = 0;
     tok.rows_are_k = true;
-    tok.alpha = alpha;
-    tok.alpha_dev = alpha_dev;
-    gemm_bf16_tokens(gv, x.narrow(0, c0, rows), *dw, true, true, !first, tok);
+    gemm_bf16_wide(gv, x.narrow(0, c0, rows), *dw, true, c0 > 0, nullptr, tok);
   }
 }
 
@@ -1041,7 +975,7 @@ ForwardOut head_forward(const at::Tensor& hidden, const at::Tensor& weight, cons
                             static_cast<size_t>(p.n_tiles) * sizeof(float), hd.stream>>>(r);
     NTB_LAUNCH_CHECK(1);
     chunk_grads(hd, x, g, st, c0, rows, tau, &st.v.head->inv, need_dh ? &out.dh : nullptr,
-                need_dw ? &out.dw : nullptr, c0 == 0, false);
+                need_dw ? &out.dw : nullptr);
   }
   return out;
 }
@@ -1067,7 +1001,8 @@ std::pair<at::Tensor, at::Tensor> head_backward(const at::Tensor& hidden, const 
     if (need_dw) dw.zero_();
     return {dh, dw};
   }
-  auto x = gather(hd, st, nullptr, 0, 0, false, nullptr, 0.f, nullptr, true);
+  auto x = gather(hd, st, nullptr, 0, 0, false, nullptr, 0.f,
+                  need_dh ? reinterpret_cast<bf16*>(dh.data_ptr()) : nullptr, true);
   auto g = at::empty({round_up(rows_max, 64), hd.ldg()}, hd.h.options());
   for (int64_t c0 = 0; c0 < hd.T; c0 += rows_max) {
     const int64_t rows = std::min(rows_max, hd.T - c0);
@@ -1083,7 +1018,7 @@ std::pair<at::Tensor, at::Tensor> head_backward(const at::Tensor& hidden, const 
     head_fix_kernel<<<static_cast<unsigned>(round_up(rows, 64)), st.K >= 128 ? 128 : 64, 0, hd.stream>>>(
         r, row_scale.data_ptr<float>());
     NTB_LAUNCH_CHECK(1);
-    chunk_grads(hd, x, g, st, c0, rows, 1.0, nullptr, need_dh ? &dh : nullptr, need_dw ? &dw : nullptr, c0 == 0, true);
+    chunk_grads(hd, x, g, st, c0, rows, 1.0, nullptr, need_dh ? &dh : nullptr, need_dw ? &dw : nullptr);
   }
   return {dh, dw};
 }

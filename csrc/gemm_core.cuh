@@ -266,16 +266,17 @@ __device__ __forceinline__ TileInfo tile_info(const GemmParams& p, int tile, int
 // thread: `begin` runs before the tile's accumulator is waited for (so it overlaps the main loop), `tile` with the
 // accumulator in TMEM. m0: first row of the warp's 32; n0: first column of the tile; Params derives from
 // GemmParams; kWarps (4 or 8) warps share the 32 KB of staging. With 8, the second four take the tile's columns
-// from BN / 2 on (`part` 1).
+// from BN / 2 on (`part` 1). `release()` is called once by the whole warp when it has read its accumulator.
 struct StoreEpilogue {
   using Params = GemmParams;
   static constexpr int kWarps = 4;
   __device__ __forceinline__ StoreEpilogue(const Params&) {}
   __device__ __forceinline__ void begin(const Params&, long, int) {}
-  template <int BN>
+  template <int BN, class Release>
   __device__ __forceinline__ void tile(uint32_t t_row, float* stage, const Params& p, long m0, int n0, bool vec_ok,
-                                       long m_end, int) {
+                                       long m_end, int, Release release) {
     epilogue_tile<BN>(t_row, stage, p, m0, n0, vec_ok, m_end, p.splits > 1);
+    release();
   }
 };
 
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 32 * Epi::kWarps);
+      mbar_init(&tempty[b], Epi::kWarps);
     }
     mbar_init(drain, 1);
     mbar_fence_init();
@@ -444,17 +445,22 @@ __global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
       if (!mbar_wait_warp(&tfull[acc], acc_phase, p.status, kStatusTimeoutEpilogue)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[acc]);
+      };
       if constexpr (GM != 2) {
-        epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, epart);
-      } else if (ti.nkb > 0) {
+        epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, epart, release);
+      } else {
         // Expert block: rows [group * M, group * M + M) of the stacked output; an expert without
         // rows contributes nothing (its accumulator was never written).
         const long base = static_cast<long>(ti.group) * (p.c_group_stride > 0 ? p.c_group_stride : p.M);
-        epilogue_tile<BN>(t_row, stage, p, base + static_cast<long>(ti.mb) * BM + q * 32, ti.nb * BN, vec_ok,
-                          base + p.M);
+        if (ti.nkb > 0)
+          epilogue_tile<BN>(t_row, stage, p, base + static_cast<long>(ti.mb) * BM + q * 32, ti.nb * BN, vec_ok,
+                            base + p.M);
+        release();
       }
-      tc_fence_before();
-      mbar_arrive(&tempty[acc]);
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
@@ -537,7 +543,7 @@ __global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 2 * 32 * Epi::kWarps);  // every epilogue thread of both CTAs
+      mbar_init(&tempty[b], 2 * Epi::kWarps);  // every epilogue warp of both CTAs
     }
     mbar_init(drain, 1);
     mbar_fence_init();
@@ -676,9 +682,12 @@ __global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
       if (!mbar_wait_warp(&tfull[acc], acc_phase, p.status, kStatusTimeoutEpilogue)) break;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
-      epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, epart);
-      tc_fence_before();
-      mbar_arrive_cluster(tempty0 + 8u * static_cast<uint32_t>(acc));
+      // One arrival a warp: CTA 0's barrier is remote for the other CTA, and 32 arrivals took 2000 clocks.
+      epi.template tile<BN>(t_row, stage, p, m0, ti.nb * BN, vec_ok, M, epart, [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * static_cast<uint32_t>(acc));
+      });
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }

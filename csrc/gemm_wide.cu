@@ -7,8 +7,8 @@
 // against one B, 48 KB for 1024 clocks, a quarter less (counted by ncu at 6144 x 4096 x 32768: 12.9 GB through the
 // crossbar before, 9.7 GB now). They fill the 512 TMEM columns, so there is no second buffer; instead the halves
 // take turns: the MMA warp runs two K blocks on half 0, then the same two on half 1, which lets half 0 be drained
-// while half 1 finishes its tile, and half 1 while half 0 begins the next one. Eight epilogue warps drain a half in
-// about the 1024 clocks of such a turn.
+// while half 1 finishes its tile, and half 1 while half 0 begins the next one. Eight epilogue warps take a half out
+// of TMEM in about the 1024 clocks of such a turn.
 //
 // Tiles rarely fill the pairs a whole number of times, and for how many tokens only the device knows. The whole
 // waves are run as they are; the tiles that remain are cut into K slices (plan_units) whose fp32 partials a second
@@ -43,7 +43,6 @@ constexpr int kMinSliceBlocks = 4;
 struct WideParams : GemmParams {
   const int* map;  // row of C for each row of the product, or nullptr
   float* ws;       // [parts, 512, 256]
-  int group;       // M tiles of a group of the tile order
 };
 
 // Units of a launch: `whole` tiles at full K, then `rest` tiles cut into `slices` of `per` K blocks.
@@ -73,14 +72,7 @@ struct Unit {
   int mb, nb, kb0, nkb, halves, part;  // part: its partial's index, -1 for a whole tile
 };
 
-__device__ __forceinline__ void wide_tile_coords(int tile, int num_m, int num_n, int group, int& mb, int& nb) {
-  const int per_group = group * num_n, g = tile / per_group, first = g * group;
-  const int gm = min(group, num_m - first), r = tile - g * per_group;
-  mb = first + r % gm;
-  nb = r / gm;
-}
-
-__device__ __forceinline__ Unit wide_unit(const Plan& pl, int u, int M, int num_m, int num_n, int nkb, int group) {
+__device__ __forceinline__ Unit wide_unit(const Plan& pl, int u, int M, int num_n, int nkb) {
   Unit t;
   int tile = u;
   t.kb0 = 0;
@@ -93,7 +85,10 @@ __device__ __forceinline__ Unit wide_unit(const Plan& pl, int u, int M, int num_
     t.kb0 = slice * pl.per;
     t.nkb = min(pl.per, nkb - t.kb0);
   }
-  wide_tile_coords(tile, num_m, num_n, group, t.mb, t.nb);
+  // N fastest: neighbouring pairs share a panel of A, all share those of B (G 6144 x 128256: 4.45 ms for dH and 4.93
+  // for dW; with blocks of 5 x 16 tiles, M fastest, 4.81 and 4.98).
+  t.mb = tile / num_n;
+  t.nb = tile - t.mb * num_n;
   t.halves = t.mb * kTileM + 2 * WideCfg::BM < M ? 2 : 1;  // no rows in the second half: not computed
   return t;
 }
@@ -126,67 +121,54 @@ __device__ __forceinline__ void wide_put(uint8_t* stage, int chunk, uint32_t a, 
   *reinterpret_cast<uint4*>(stage + lane * 128 + ((chunk ^ (lane & 7)) * 16)) = make_uint4(a, b, c, d);
 }
 
-// One warp's 32 rows x 128 columns of a half. m0, n0: its first row and column in the product.
-__device__ __forceinline__ void wide_store(uint32_t t_row, uint8_t* stage, const WideParams& p, const Unit& u, int M,
-                                           int m0, int n0, float alpha) {
-  const int cols = min(128, p.N - n0);  // a multiple of 8
+// One warp's 32 rows x 64 columns, in registers. m0, n0: first row and column in the product; mine: the byte offset of
+// this lane's row in C (column n0 - skip), -1 for none.
+__device__ __forceinline__ void wide_store(uint32_t (&r)[2][32], uint8_t* stage, const WideParams& p, const Unit& u,
+                                           int M, int m0, int n0, long mine, int skip, float alpha) {
+  const int cols = min(64, p.N - n0);  // a multiple of 8
   if (cols <= 0) return;
   if (u.part >= 0) {
-    float* ws = p.ws + static_cast<long>(u.part) * kTileM * kTileN;
-    const int r0 = m0 - u.mb * kTileM, c0 = n0 - u.nb * kTileN;
-#pragma unroll 1
-    for (int g = 0; g < cols; g += 32) {
-      uint32_t r[32];
-      tmem_ld32(t_row + g, r);
+    float* ws = p.ws + static_cast<long>(u.part) * kTileM * kTileN + (m0 - u.mb * kTileM) * kTileN + n0 - u.nb * kTileN;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) wide_put(stage, c, r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+    for (int g = 0; g < 2; ++g) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) wide_put(stage, c, r[g][4 * c], r[g][4 * c + 1], r[g][4 * c + 2], r[g][4 * c + 3]);
       wide_flush<false>(stage, [&](int row) -> uint8_t* {
-        return m0 + row < M ? reinterpret_cast<uint8_t*>(ws + static_cast<long>(r0 + row) * kTileN + c0 + g) : nullptr;
+        return m0 + row < M ? reinterpret_cast<uint8_t*>(ws + row * kTileN + g * 32) : nullptr;
       }, 128);
     }
     return;
   }
-  auto c_row = [&](int row) -> long {
-    const int m = m0 + row;
-    if (m >= M) return -1;
-    return (p.map != nullptr ? __ldg(p.map + m) : m) * p.ldc + n0;
+  auto row_ptr = [&](int row, int byte) -> uint8_t* {
+    const long at = __shfl_sync(0xffffffffu, mine, row);
+    return at >= 0 ? reinterpret_cast<uint8_t*>(p.C) + at + byte : nullptr;
   };
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int c = 0; c < 32; ++c) r[g][c] = __float_as_uint(__uint_as_float(r[g][c]) * alpha);
   if (p.c_f32) {
-    float* C = reinterpret_cast<float*>(p.C);
-#pragma unroll 1
-    for (int g = 0; g < cols; g += 32) {
-      uint32_t r[32];
-      tmem_ld32(t_row + g, r);
 #pragma unroll
-      for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * alpha);
+    for (int g = 0; g < 2; ++g) {
+      if (g * 32 >= cols) break;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) wide_put(stage, c, r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
-      auto ptr = [&](int row) -> uint8_t* {
-        const long at = c_row(row);
-        return at >= 0 ? reinterpret_cast<uint8_t*>(C + at + g) : nullptr;
-      };
-      if (p.accumulate) wide_flush<true>(stage, ptr, (cols - g) * 4);
-      else wide_flush<false>(stage, ptr, (cols - g) * 4);
+      for (int c = 0; c < 8; ++c) wide_put(stage, c, r[g][4 * c], r[g][4 * c + 1], r[g][4 * c + 2], r[g][4 * c + 3]);
+      auto ptr = [&](int row) { return row_ptr(row, (skip + g * 32) * 4); };
+      if (p.accumulate) wide_flush<true>(stage, ptr, (cols - g * 32) * 4);
+      else wide_flush<false>(stage, ptr, (cols - g * 32) * 4);
     }
   } else {
-    __nv_bfloat16* C = reinterpret_cast<__nv_bfloat16*>(p.C);
-#pragma unroll 1
-    for (int g = 0; g < cols; g += 64) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t r[32], w[16];
-        tmem_ld32(t_row + g + half * 32, r);
+    for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          w[j] = pack_bf16x2(__uint_as_float(r[2 * j]) * alpha, __uint_as_float(r[2 * j + 1]) * alpha);
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) wide_put(stage, half * 4 + c, w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+        for (int k = 0; k < 4; ++k)
+          w[k] = pack_bf16x2(__uint_as_float(r[g][8 * c + 2 * k]), __uint_as_float(r[g][8 * c + 2 * k + 1]));
+        wide_put(stage, g * 4 + c, w[0], w[1], w[2], w[3]);
       }
-      wide_flush<false>(stage, [&](int row) -> uint8_t* {
-        const long at = c_row(row);
-        return at >= 0 ? reinterpret_cast<uint8_t*>(C + at + g) : nullptr;
-      }, (cols - g) * 2);
-    }
+    wide_flush<false>(stage, [&](int row) { return row_ptr(row, skip * 2); }, cols * 2);
   }
 }
 
@@ -257,7 +239,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
     bool ok = true;
     const uint32_t expect = rank == 0 ? 1u : 0u;
     for (int i = pair; i < units && ok; i += npairs) {
-      const Unit u = wide_unit(pl, i, M, num_m, num_n, nkb, p.group);
+      const Unit u = wide_unit(pl, i, M, num_n, nkb);
       const int arow = u.mb * kTileM + static_cast<int>(rank) * BM;
       const int bcol = u.nb * kTileN + static_cast<int>(rank) * (BN / 2);
       const uint32_t bytes = 2u * static_cast<uint32_t>(u.halves * Cfg::HALF_BYTES + Cfg::B_BYTES);
@@ -335,7 +317,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
       };
       bool ok = true;
       for (int i = pair; i < units && ok; i += npairs) {
-        const Unit u = wide_unit(pl, i, M, num_m, num_n, nkb, p.group);
+        const Unit u = wide_unit(pl, i, M, num_n, nkb);
         const bool two = u.halves == 2;
         for (int kb = 0; kb < u.nkb; kb += 2) {
           const bool both = kb + 1 < u.nkb, last = kb + 2 >= u.nkb;
@@ -392,7 +374,7 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
     uint32_t uses[2] = {0, 0};
     bool ok = true;
     for (int i = pair; i < units && ok; i += npairs) {
-      const Unit u = wide_unit(pl, i, M, num_m, num_n, nkb, p.group);
+      const Unit u = wide_unit(pl, i, M, num_n, nkb);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (h >= u.halves) break;
@@ -402,12 +384,23 @@ __global__ void __launch_bounds__(WideCfg::THREADS, 1)
         }
         ++uses[h];
         tc_fence_after();
-        wide_store(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(h * BN + epart * 128),
-                   stage, p, u, M, u.mb * kTileM + h * 2 * BM + static_cast<int>(rank) * BM + q * 32,
-                   u.nb * kTileN + epart * 128, alpha);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * static_cast<uint32_t>(h));
+        const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(h * BN + epart * 128);
+        const int m0 = u.mb * kTileM + h * 2 * BM + static_cast<int>(rank) * BM + q * 32;
+        const int n0 = u.nb * kTileN + epart * 128, m = m0 + lane;
+        long mine = -1;
+        if (m < M) mine = ((p.map != nullptr ? __ldg(p.map + m) : m) * p.ldc + n0) * (p.c_f32 ? 4 : 2);
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 64) {
+          uint32_t r[2][32];
+          tmem_ld32(t_row + c, r[0]);
+          tmem_ld32(t_row + c + 32, r[1]);
+          if (c == 64) {  // the half is free again before its last columns are stored
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * static_cast<uint32_t>(h));
+          }
+          wide_store(r, stage, p, u, M, m0, n0 + c, mine, c, alpha);
+        }
       }
     }
   }
@@ -429,8 +422,7 @@ __global__ void __launch_bounds__(256) gemm_wide_join_kernel(WideParams p, int p
   const Plan pl = plan_units(num_m * num_n, (K + WideCfg::BK - 1) / WideCfg::BK, pairs);
   const int r = blockIdx.x;
   if (r >= pl.rest) return;
-  int mb, nb;
-  wide_tile_coords(pl.whole + r, num_m, num_n, p.group, mb, nb);
+  const int mb = (pl.whole + r) / num_n, nb = pl.whole + r - mb * num_n;
   const int col = (threadIdx.x & 63) * 4, n = nb * kTileN + col;
   if (n >= p.N) return;
   const float alpha = p.alpha_dev != nullptr ? p.alpha * __ldg(p.alpha_dev) : p.alpha;
@@ -533,10 +525,7 @@ void gemm_bf16_wide(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, b
   p.rows_are_k = tok.rows_are_k ? 1 : 0;
   p.map = map;
   const int pairs = num_sms(a.get_device()) / 2;
-  // A wave of pairs covers whole rows of tiles where N is narrow enough (A is then read from DRAM once and the B
-  // panels stay in L2), a block of 6 x 12 tiles otherwise.
   const int64_t num_n = (N + kTileN - 1) / kTileN, num_m = (M + kTileM - 1) / kTileM;
-  p.group = static_cast<int>(num_n <= 18 ? (pairs + num_n - 1) / num_n : 6);
   // Partial tiles: what the plan can ask for at most, over all token counts.
   const int64_t nkb = (K + WideCfg::BK - 1) / WideCfg::BK;
   const int64_t rest = std::min<int64_t>(pairs - 1, num_m * num_n);

@@ -122,20 +122,23 @@ struct HeadEpilogue {
           make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
   }
   __device__ __forceinline__ void flush(const uint8_t* stage, const Params& p, long m0, int col, long m_end) {
-    const int lane = threadIdx.x & 31, ch = lane & 7;
+    const int lane = threadIdx.x & 31, ch = lane & 7, row0 = lane >> 3;
+    const int rows = static_cast<int>(m_end - m0) - row0;  // of this lane's, every fourth
+    uint16_t* dst = p.codes + (m0 + row0) * p.ldg + col + ch * 8;
     __syncwarp();
+    uint4 v[8];
 #pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const int row = it * 4 + (lane >> 3);
-      const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 128 + ((ch ^ (row & 7)) * 16));
-      if (m0 + row < m_end) *reinterpret_cast<uint4*>(p.codes + (m0 + row) * p.ldg + col + ch * 8) = v;
-    }
+    for (int it = 0; it < 8; ++it)
+      v[it] = *reinterpret_cast<const uint4*>(stage + (it * 4 + row0) * 128 + ((ch ^ ((it * 4 + row0) & 7)) * 16));
+#pragma unroll
+    for (int it = 0; it < 8; ++it, dst += 4 * p.ldg)
+      if (it * 4 < rows) *reinterpret_cast<uint4*>(dst) = v[it];
     __syncwarp();
   }
 
-  template <int BN>
+  template <int BN, class Release>
   __device__ __forceinline__ void tile(uint32_t t_row, float* stage_f, const Params& p, long m0, int n0, bool,
-                                       long m_end, int part) {
+                                       long m_end, int part, Release release) {
     constexpr int COLS = BN / 2, GROUPS = COLS / 32;
     uint8_t* stage = reinterpret_cast<uint8_t*>(stage_f);
     const int lane = threadIdx.x & 31;
@@ -158,10 +161,12 @@ struct HeadEpilogue {
         }
         flush(stage, p, m0, n0 + g, m_end);
       }
+      release();
     } else {
       uint32_t r[GROUPS][32];
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) tmem_ld32(t_row + g * 32, r[g]);
+      release();
       if (ncol < COLS) {  // the vocabulary ends in here
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g)

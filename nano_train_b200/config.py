@@ -88,6 +88,11 @@ class ModelConfig:
     tie_word_embeddings: bool = True
     sequence_parallel: bool = False
     init_std: float = 0.02
+    # Vocabulary ends. None: plain lookup; a number multiplies the embedded tokens and takes the lookup whose weight
+    # gradient is summed in a fixed order (ops.scaled_embedding).
+    embedding_scale: Optional[float] = None
+    # The training loss without materialised logits (ops.linear_cross_entropy); False keeps the logits.
+    fused_head_loss: bool = False
 
 
 @dataclass

@@ -235,12 +235,14 @@ class RMSNorm(ModulePrecisionStateMixin, nn.Module):
 
 
 class Embedding(ModulePrecisionStateMixin, nn.Module):
-    """Token lookup table [num_embeddings, dim] ~ N(0, 0.02)."""
+    """Token lookup table [num_embeddings, dim] ~ N(0, 0.02). With a ``scale`` the rows are multiplied by it and the
+    weight gradient is summed over tokens sorted by id (``ops.scaled_embedding``)."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, *, param_dtype: torch.dtype = torch.float32,
                  param_device: Optional[torch.device] = None, module_path: str = "embedding",
-                 precision_resolver=None, init_std: float = 0.02):
+                 precision_resolver=None, init_std: float = 0.02, scale: Optional[float] = None):
         super().__init__()
+        self.scale = scale
         self.num_embeddings = num_embeddings
         self.embedding_dim = embedding_dim
         self.weight = nn.Parameter(torch.empty(num_embeddings, embedding_dim, dtype=param_dtype,
@@ -251,6 +253,8 @@ class Embedding(ModulePrecisionStateMixin, nn.Module):
                                           precision_resolver=_resolver(precision_resolver))
 
     def forward(self, indices: torch.Tensor) -> torch.Tensor:
+        if self.scale is not None:
+            return ops.scaled_embedding(indices, self.weight, self.scale)
         return ops.embedding(indices, self.weight)
 
 
@@ -264,8 +268,9 @@ class VocabParallelEmbedding(ModulePrecisionStateMixin, nn.Module):
     def __init__(self, num_embeddings: int, embedding_dim: int, tp_rank: int = 0, tp_size: int = 1, tp_group=None,
                  *, param_dtype: torch.dtype = torch.float32, param_device: Optional[torch.device] = None,
                  module_path: str = "embedding", precision_resolver=None, sequence_parallel: bool = False,
-                 init_std: float = 0.02):
+                 init_std: float = 0.02, scale: Optional[float] = None):
         super().__init__()
+        self.scale = scale
         if num_embeddings % tp_size != 0:
             raise ValueError(f"vocab {num_embeddings} must be divisible by tp_size {tp_size}")
         self.num_embeddings = num_embeddings
@@ -284,7 +289,10 @@ class VocabParallelEmbedding(ModulePrecisionStateMixin, nn.Module):
                                           precision_resolver=_resolver(precision_resolver))
 
     def forward(self, indices: torch.Tensor) -> torch.Tensor:
-        out = ops.embedding(indices, self.weight, self.vocab_start)
+        if self.scale is not None:
+            out = ops.scaled_embedding(indices, self.weight, self.scale, vocab_start=self.vocab_start)
+        else:
+            out = ops.embedding(indices, self.weight, self.vocab_start)
         if self.tp_size == 1:
             return out
         if self.sequence_parallel:

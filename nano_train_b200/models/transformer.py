@@ -246,10 +246,11 @@ class TransformerModel(nn.Module):
             self.token_embeddings = VocabParallelEmbedding(config.vocab_size, config.hidden_size, self.tp_rank,
                                                            self.tp_size, self.tp_group, module_path="token_embeddings",
                                                            sequence_parallel=self.sequence_parallel,
-                                                           init_std=config.init_std, **common)
+                                                           init_std=config.init_std, scale=config.embedding_scale,
+                                                           **common)
         else:
             self.token_embeddings = Embedding(config.vocab_size, config.hidden_size, module_path="token_embeddings",
-                                              init_std=config.init_std, **common)
+                                              init_std=config.init_std, scale=config.embedding_scale, **common)
         if config.position == "learned":
             self.position_embeddings = Embedding(config.max_position_embeddings, config.hidden_size,
                                                  module_path="position_embeddings", init_std=config.init_std,
@@ -349,13 +350,46 @@ class TransformerModel(nn.Module):
 
         Under TP the LM head stays vocab-sharded and the loss is the
         vocab-parallel cross-entropy (three [T] all-reduces), and the
-        gradient is written over the logits buffer in place.
+        gradient is written over the logits buffer in place. With
+        ``config.fused_head_loss`` the head and its loss are one operator and
+        no logits are kept.
         """
         h = self.hidden_states(input_ids)
-        logits = self.lm_head(h)
         group = self.tp_group if self.tp_enabled else None
+        if self.config.fused_head_loss:
+            return ops.linear_cross_entropy(self._head_input(h), self.lm_head.weight, labels.reshape(-1),
+                                            ignore_index=ignore_index, vocab_start=self.vocab_start, group=group)
+        logits = self.lm_head(h)
         return ops.cross_entropy(logits, labels.reshape(-1), ignore_index=ignore_index, vocab_start=self.vocab_start,
                                  group=group, inplace_grad=True)
+
+    def _head_input(self, h: torch.Tensor) -> torch.Tensor:
+        """Hidden states as the fused head losses take them: every token, in the head's dtype."""
+        if self.lm_head.bias is not None:
+            raise ValueError("the fused head losses need an LM head without bias")
+        if self.lm_head._compute_lowbit_mode() is not None or self.lm_head._persistent_mode() != "off":
+            raise ValueError("the fused head losses need an LM head in full precision")
+        if self.sequence_parallel:  # the loss sums the gradient over the ranks; each keeps its tokens' rows
+            h = comm.gather_from_sequence_parallel_region(h, self.tp_rank, self.tp_size, self.tp_group, seq_dim=0)
+        return h.to(self.lm_head.weight.dtype)
+
+    def forward_distill_loss(self, input_ids: torch.Tensor, teacher_values: torch.Tensor,
+                             teacher_indices: torch.Tensor, labels: torch.Tensor | None = None, *,
+                             temperature: float = 1.0, label_weight: float = 0.5,
+                             ignore_index: int = -100) -> torch.Tensor:
+        """Distillation from a teacher's top logits [B, S, K] at every position (``ops.linear_distillation``), mixed
+        as ``(1 - label_weight) * distillation + label_weight * cross-entropy`` when ``labels`` are given. Neither
+        loss keeps logits."""
+        if self.tp_enabled:
+            raise ValueError("distillation from top logits needs the whole vocabulary on each rank (no TP)")
+        h = self._head_input(self.hidden_states(input_ids))
+        K = teacher_values.shape[-1]
+        loss = ops.linear_distillation(h, self.lm_head.weight, teacher_values.reshape(-1, K),
+                                       teacher_indices.reshape(-1, K), temperature=temperature)
+        if labels is None:
+            return loss
+        hard = ops.linear_cross_entropy(h, self.lm_head.weight, labels.reshape(-1), ignore_index=ignore_index)
+        return (1.0 - label_weight) * loss + label_weight * hard
 
     # ------------------------------------------------------------------ full <-> TP-shard state
     def shard_full_state_dict(self, full: dict) -> dict:

@@ -148,3 +148,104 @@ def test_cross_entropy_over_a_sharded_vocabulary(tmp_path):
             torch.testing.assert_close(p[reduction][0], loss.detach(), rtol=1e-5, atol=1e-6)
             torch.testing.assert_close(p[reduction][1], dh, rtol=1e-5, atol=1e-6)
         torch.testing.assert_close(torch.cat([p[reduction][2] for p in parts]), dw, rtol=1e-5, atol=1e-6)
+
+
+# ------------------------------------------------------------------------------------------------ in the model
+def _config(**kw):
+    from nano_train_b200.config import FullPrecisionResolver, ModelConfig
+
+    return ModelConfig(param_dtype=torch.float32, param_device=torch.device("cpu"),
+                       precision_resolver=FullPrecisionResolver(), hidden_size=32, num_layers=1, num_attention_heads=2,
+                       intermediate_size=48, vocab_size=40, max_position_embeddings=32, dropout=0.0, norm="rmsnorm",
+                       position="rope", mlp="swiglu", bias=False, **kw)
+
+
+def test_model_with_fused_head_loss_matches_the_one_with_logits():
+    from nano_train_b200.models.transformer import TransformerModel
+
+    for tie in (False, True):
+        torch.manual_seed(0)
+        plain = TransformerModel(_config(tie_word_embeddings=tie))
+        fused = TransformerModel(_config(tie_word_embeddings=tie, fused_head_loss=True, embedding_scale=1.0))
+        fused.load_state_dict(plain.state_dict())
+        ids = torch.randint(0, 40, (2, 9))
+        lab = torch.randint(0, 40, (2, 9))
+        lab[0, :4] = -100
+        losses = [m.forward_loss(ids, lab) for m in (plain, fused)]
+        torch.testing.assert_close(losses[1], losses[0], rtol=1e-6, atol=1e-6)
+        for loss in losses:
+            loss.backward()
+        for (name, p), q in zip(plain.named_parameters(), fused.parameters()):
+            torch.testing.assert_close(q.grad, p.grad, rtol=1e-5, atol=1e-6, msg=name)
+
+
+def test_embedding_scale_and_distillation_in_the_model():
+    from nano_train_b200.models.transformer import TransformerModel
+
+    torch.manual_seed(0)
+    m = TransformerModel(_config(tie_word_embeddings=False, embedding_scale=3.0))
+    ids = torch.randint(0, 40, (2, 9))
+    torch.testing.assert_close(m.token_embeddings(ids), 3.0 * m.token_embeddings.weight[ids])
+    logits = m(ids).detach()
+    values, indices = logits.topk(40, dim=-1)
+    assert abs(m.forward_distill_loss(ids, values, indices).item()) < 1e-5  # its own teacher
+    lab = torch.randint(0, 40, (2, 9))
+    both = m.forward_distill_loss(ids, values[..., :4], indices[..., :4], lab, label_weight=0.25)
+    want = 0.75 * m.forward_distill_loss(ids, values[..., :4], indices[..., :4]) + 0.25 * m.forward_loss(ids, lab)
+    torch.testing.assert_close(both, want, rtol=1e-5, atol=1e-6)
+
+
+def _tp_worker(rank, world, port, out):
+    import torch.distributed as dist
+
+    from nano_train_b200.config import TPConfig
+    from nano_train_b200.models.transformer import TransformerModel
+
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        torch.manual_seed(0)
+        ref = TransformerModel(_config(tie_word_embeddings=False))
+        ids, lab = torch.randint(0, 40, (2, 8)), torch.randint(0, 40, (2, 8))
+        lab[1, 2:5] = -100
+        errs = {}
+        loss = ref.forward_loss(ids, lab)
+        for sp in (False, True):
+            tp = TransformerModel(_config(tie_word_embeddings=False, sequence_parallel=sp, fused_head_loss=True,
+                                          embedding_scale=1.0),
+                                  TPConfig(enabled=True, rank=rank, size=world, group=dist.group.WORLD))
+            tp.load_full_state_dict({k: v.clone() for k, v in ref.state_dict().items()})
+            got = tp.forward_loss(ids, lab)
+            errs[f"loss{sp}"] = abs(float(got.detach()) - float(loss.detach()))
+            got.backward()
+            ref.zero_grad()
+            ref.forward_loss(ids, lab).backward()
+            shards = ref.lm_head.weight.grad.chunk(world, 0)
+            errs[f"head{sp}"] = float((tp.lm_head.weight.grad - shards[rank]).abs().max())
+            shards = ref.blocks[0].mlp.fc2.weight.grad.chunk(world, 1)
+            errs[f"fc2{sp}"] = float((tp.blocks[0].mlp.fc2.weight.grad - shards[rank]).abs().max())
+        torch.save(errs, f"{out}.{rank}")
+    finally:
+        dist.destroy_process_group()
+
+
+def test_fused_head_loss_under_tensor_parallelism(tmp_path):
+    out = str(tmp_path / "errs")
+    mp.spawn(_tp_worker, args=(2, free_port(), out), nprocs=2, join=True)
+    for r in range(2):
+        errs = torch.load(f"{out}.{r}")
+        assert max(errs.values()) < 1e-5, errs
+
+
+def test_distillation_example(tmp_path):
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+
+    p = subprocess.run([sys.executable, os.path.join(ROOT, "examples", "distill.py"), "--steps", "11"],
+                       capture_output=True, text=True, timeout=600, cwd=str(tmp_path),
+                       env=dict(os.environ, OMP_NUM_THREADS="2", PYTHONPATH=ROOT, CUDA_VISIBLE_DEVICES=""))
+    assert p.returncode == 0, p.stderr[-2000:]
+    losses = [float(line.split()[3]) for line in p.stdout.splitlines() if line.startswith("step ")]
+    assert losses[-1] < losses[0], p.stdout

@@ -333,101 +333,98 @@ __global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
+  // Both loops are run by whole warps with one elected lane, as in the CTA-pair kernel below.
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t filled_mask = 0;
-      uint32_t last_phase[STAGES];
-#pragma unroll
-      for (int s = 0; s < STAGES; ++s) last_phase[s] = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-        const TileInfo ti = tile_info<GM>(p, tile, num_m, num_n, num_kb, BM, BK);
-        const int mb = ti.mb, nb = ti.nb;
-        // Mode 1: the expert's slice of the stacked B starts at group * b_group_rows rows.
-        const int b_row0 = GM == 1 ? ti.group * p.b_group_rows : 0;
-        for (int kq = 0; kq < ti.nkb; ++kq) {
-          const int kb = ti.kb0 + kq;
-          if (!mbar_wait(&empty[stage], phase ^ 1, p.status, kStatusTimeoutProducer)) {
-            ok = false;
-            break;
-          }
+    const bool leader = elect_one();
+    uint32_t stage = 0, phase = 0, filled = 0, last = 0;  // bit s: stage s was filled, in that phase
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      const TileInfo ti = tile_info<GM>(p, tile, num_m, num_n, num_kb, BM, BK);
+      const int arow = ti.mb * BM, bcol = ti.nb * BN;
+      // Mode 1: the expert's slice of the stacked B starts at group * b_group_rows rows.
+      const int b_row0 = GM == 1 ? ti.group * p.b_group_rows : 0;
+      int k0 = ti.kb0 * BK;
+      for (int kq = 0; kq < ti.nkb; ++kq, k0 += BK) {
+        if (!mbar_wait_warp(&empty[stage], phase ^ 1, p.status, kStatusTimeoutProducer)) {
+          ok = false;
+          break;
+        }
+        if (leader) {
           mbar_expect_tx(&full[stage], A_BYTES + B_BYTES);
           uint8_t* a_dst = sA + stage * A_BYTES;
           uint8_t* b_dst = sB + stage * B_BYTES;
           if constexpr (!A_MN) {
-            tma_load_2d(a_dst, &tmA, &full[stage], kb * BK, mb * BM);
+            tma_load_2d(a_dst, &tmA, &full[stage], k0, arow);
           } else {
 #pragma unroll
-            for (int j = 0; j < BM / 64; ++j) tma_load_2d(a_dst + j * 8192, &tmA, &full[stage], mb * BM + j * 64, kb * BK);
+            for (int j = 0; j < BM / 64; ++j) tma_load_2d(a_dst + j * 8192, &tmA, &full[stage], arow + j * 64, k0);
           }
           if constexpr (!B_MN) {
-            tma_load_2d(b_dst, &tmB, &full[stage], kb * BK, b_row0 + nb * BN);
+            tma_load_2d(b_dst, &tmB, &full[stage], k0, b_row0 + bcol);
           } else {
 #pragma unroll
             for (int j = 0; j < BN / 64; ++j)
-              tma_load_2d(b_dst + j * 8192, &tmB, &full[stage], nb * BN + j * 64, b_row0 + kb * BK);
-          }
-          filled_mask |= 1u << stage;
-          last_phase[stage] = phase;
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
+              tma_load_2d(b_dst + j * 8192, &tmB, &full[stage], bcol + j * 64, b_row0 + k0);
           }
         }
+        __syncwarp();
+        filled |= 1u << stage;
+        last = (last & ~(1u << stage)) | (phase << stage);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
-      // Never leave the CTA with a TMA write still landing in shared memory.
-      for (int s = 0; s < STAGES; ++s)
-        if (filled_mask & (1u << s)) mbar_wait(&full[s], last_phase[s], nullptr, 0) || true;
     }
+    // Never leave the CTA with a TMA write still landing in shared memory.
+    for (int s = 0; s < STAGES; ++s)
+      if (filled >> s & 1u) mbar_wait(&full[s], last >> s & 1u, nullptr, 0);
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int acc = 0;
-      uint32_t acc_phase = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-        const int tile_nkb =
-            (GM == 2 || (GM == 0 && p.splits > 1)) ? tile_info<GM>(p, tile, num_m, num_n, num_kb, BM, BK).nkb : num_kb;
-        if (!mbar_wait(&tempty[acc], acc_phase ^ 1, p.status, kStatusTimeoutMma)) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-        for (int kb = 0; kb < tile_nkb; ++kb) {
-          if (!mbar_wait(&full[stage], phase, p.status, kStatusTimeoutMma)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a_base = smem_u32(sA + stage * A_BYTES);
-          const uint32_t b_base = smem_u32(sB + stage * B_BYTES);
-#pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            // K-major: advance 16 elements (32 B) inside the 128 B swizzle row.
-            // MN-major: advance 16 K-rows (16 x 128 B) = two 8-row swizzle atoms.
-            const uint64_t adesc = A_MN ? make_smem_desc_sw128(a_base + k * 2048, 8192, 1024)
-                                        : make_smem_desc_sw128(a_base + k * 32, 16, 1024);
-            const uint64_t bdesc = B_MN ? make_smem_desc_sw128(b_base + k * 2048, 8192, 1024)
-                                        : make_smem_desc_sw128(b_base + k * 32, 16, 1024);
-            umma_f16_ss(d_tmem, adesc, bdesc, IDESC, (kb | k) != 0 ? 1u : 0u);
-          }
-          umma_commit(&empty[stage]);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
+    // K-major: 16 elements (32 B) further inside the 128 B swizzle row; MN-major: 16 K rows of 128 B.
+    constexpr uint32_t A_K = (A_MN ? 2048 : 32) >> 4, B_K = (B_MN ? 2048 : 32) >> 4;
+    const bool leader = elect_one();
+    const uint64_t a0 = make_smem_desc_sw128(smem_u32(sA), A_MN ? 8192 : 16, 1024);
+    const uint64_t b0 = make_smem_desc_sw128(smem_u32(sB), B_MN ? 8192 : 16, 1024);
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+    uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      const int tile_nkb =
+          (GM == 2 || (GM == 0 && p.splits > 1)) ? tile_info<GM>(p, tile, num_m, num_n, num_kb, BM, BK).nkb : num_kb;
+      if (!mbar_wait_warp(&tempty[acc], acc_phase ^ 1, p.status, kStatusTimeoutMma)) break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem + acc * BN;
+      for (int kb = 0; kb < tile_nkb; ++kb) {
+        if (!mbar_wait_warp(&full[stage], phase, p.status, kStatusTimeoutMma)) {
+          ok = false;
+          break;
         }
-        if (!ok) break;
-        umma_commit(&tfull[acc]);
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1;
+        tc_fence_after();
+        const uint64_t a = a0 + stage * static_cast<uint32_t>(A_BYTES >> 4);
+        const uint64_t b = b0 + stage * static_cast<uint32_t>(B_BYTES >> 4);
+        if (leader) {
+          umma_f16_ss(d_tmem, a, b, IDESC, kb != 0 ? 1u : 0u);
+#pragma unroll
+          for (int k = 1; k < BK / 16; ++k) umma_f16_ss(d_tmem, a + k * A_K, b + k * B_K, IDESC, 1u);
+          umma_commit(&empty[stage]);
+        }
+        __syncwarp();
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
-      // Make sure every MMA this thread issued has retired before TMEM is freed.
-      if (static_cast<int>(blockIdx.x) < num_tiles) {
-        umma_commit(drain);
-        mbar_wait(drain, 0, nullptr, 0);
-      }
+      if (!ok) break;
+      if (leader) umma_commit(&tfull[acc]);
+      __syncwarp();
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    // Make sure every MMA this warp issued has retired before TMEM is freed.
+    if (static_cast<int>(blockIdx.x) < num_tiles) {
+      if (leader) umma_commit(drain);
+      __syncwarp();
+      mbar_wait(drain, 0, nullptr, 0);
     }
   } else {
     // Epilogue: warps 2..5 -> TMEM lane quarter (warp % 4).

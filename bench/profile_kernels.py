@@ -25,6 +25,9 @@ L2 where the kernel is bandwidth-bound), runs 2 warm-up launches and then
   mla_k         MLA key assembly [k_nope | rope(k_rope)], DeepSeek-V2-Lite micro-batch (8192 tokens, 16 heads,
                 nope 128 / rope 64 / v 128, kv_lora 512); mla_k_bwd its backward
   ce            vocab cross-entropy stats+bwd 4096 x 32064
+  linear_ce     linear-head cross-entropy with its gradients, 2048 tokens x 4096, vocabulary 32768
+  linear_kd     the same as a distillation from 64 teacher logits a token
+  embedding     scaled embedding and its sorted gradient, 32768 tokens x 4096, vocabulary 32768
   router        fused top-k router fwd, 16384 tokens x 64 experts, top-6 softmax (bf16)
   router_bwd    its backward
   ep_layer      expert-parallel dispatch -> receive plan -> gather -> pull-combine of one MoE layer
@@ -204,6 +207,34 @@ def main():
         logits = torch.randn(4096, 32064, **bf)
         labels = torch.randint(0, 32064, (4096,), device=dev)
         fn = lambda: C.ce_stats(logits, labels, 0, -100)  # noqa: E731
+    elif a.case in ("linear_ce", "linear_kd"):
+        from nano_train_b200 import ops
+
+        T, H, V = 2048, 4096, 32768
+        h = torch.randn(T, H, device=dev).bfloat16().requires_grad_(True)
+        w = (torch.randn(V, H, device=dev) * 0.02).bfloat16().requires_grad_(True)
+        lab = torch.randint(0, V, (T,), device=dev)
+        idx = torch.arange(64, device=dev) * 512 + torch.randint(0, 512, (T, 64), device=dev)
+        val = torch.randn(T, 64, device=dev)
+        nflops = 6 * T * H * V
+
+        def run():
+            loss = (ops.linear_cross_entropy(h, w, lab) if a.case == "linear_ce" else
+                    ops.linear_distillation(h, w, val, idx, temperature=2.0))
+            torch.autograd.grad(loss, (h, w))
+        fn = run
+    elif a.case == "embedding":
+        from nano_train_b200 import ops
+
+        T, H, V = 32768, 4096, 32768
+        w = torch.randn(V, H, device=dev).bfloat16().requires_grad_(True)
+        ids = (V ** torch.rand(T, device=dev)).long().clamp_(0, V - 1)
+        dout = torch.randn(T, H, device=dev).bfloat16()
+        nbytes = 2 * H * (3 * T + V)
+
+        def run():
+            torch.autograd.grad(ops.scaled_embedding(ids, w, 64.0), (w,), dout)
+        fn = run
     elif a.case in ("router", "router_bwd"):
         logits = torch.randn(16384, 64, **bf)
         cfg = (6, True, 1, 1, True, 1.0)

@@ -65,7 +65,7 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
     embed_gather_kernel(const int64_t* __restrict__ ids, const T* __restrict__ w, int64_t n, int H, int64_t V,
                         int64_t vstart, float scale, T* __restrict__ out) {
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 2;  // 66 us at 32768 x 4096; 4: 72 us, 8: 92 us (fewer warps resident)
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (t >= n) return;
   const int lane = threadIdx.x & 31;
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kSortThreads)
 }
 
 // ------------------------------------------------------------------ sums over runs of equal ids
-constexpr int kPieceMax = 64;
+constexpr int kPiece = 32;  // sorted tokens of a CTA (64: 9 us more at 32768 x 4096, 16: 17 us more partials)
 constexpr int kSumThreads = 128;
 constexpr int kZeroRows = 32;  // vocabulary rows (a word of the bitmap) whose zeros one CTA writes
 
@@ -297,7 +297,6 @@ struct SumParams {
   int64_t V;
   int H;
   float scale;
-  int piece;   // sorted tokens of a CTA, up to kPieceMax
   int pieces, slices;  // slices of VEC * kSumThreads columns
   const unsigned* present;
   float* part;  // [pieces, 2, H] partial sums: 0 the run that came in, 1 the run that goes on
@@ -340,12 +339,12 @@ __device__ __forceinline__ void write_row(G* dw, float scale, float (&acc)[VEC])
   else RowVec<G, VEC>::store(dw, acc);
 }
 
-// pieces * slices CTAs sum `piece` sorted tokens each over one slice of the columns; without ADD the others, spread
+// pieces * slices CTAs sum kPiece sorted tokens each over one slice of the columns; without ADD the others, spread
 // evenly among them because they only write, zero the rows that no token has.
 template <typename T, typename G, int VEC, bool ADD>
 __global__ void __launch_bounds__(kSumThreads)
     embed_sum_kernel(SumParams p, const T* __restrict__ dout, G* __restrict__ dw) {
-  __shared__ int2 items[kPieceMax + 2];
+  __shared__ int2 items[kPiece + 2];
   const unsigned sums = p.pieces * p.slices;
   const unsigned block = static_cast<unsigned>(static_cast<uint64_t>(blockIdx.x) * sums / gridDim.x);
   if (static_cast<unsigned>((static_cast<uint64_t>(blockIdx.x) + 1) * sums / gridDim.x) == block) {
@@ -365,7 +364,7 @@ __global__ void __launch_bounds__(kSumThreads)
   }
   const int piece = block / p.slices;
   const int col = ((block - piece * p.slices) * kSumThreads + threadIdx.x) * VEC;
-  const int i0 = piece * p.piece, m = min(p.piece, p.n - i0);
+  const int i0 = piece * kPiece, m = min(kPiece, p.n - i0);
   // items[1 + i] is sorted token i0 + i; the neighbours' ids tell which runs cross the ends.
   for (int i = threadIdx.x; i < m + 2; i += kSumThreads) {
     const int at = i0 + i - 1;
@@ -407,7 +406,7 @@ __global__ void __launch_bounds__(kSumThreads)
 // Joins the runs that cross pieces: the CTA of the piece where a run begins adds the later pieces' partials.
 template <typename G, int VEC, bool ADD>
 __global__ void __launch_bounds__(kSumThreads) embed_join_kernel(SumParams p, G* __restrict__ dw) {
-  const int piece = blockIdx.x, first = piece * p.piece, last = first + p.piece - 1;
+  const int piece = blockIdx.x, first = piece * kPiece, last = first + kPiece - 1;
   if (last + 1 >= p.n) return;
   const int id = __ldg(&p.sorted[last].x), after = __ldg(&p.sorted[last + 1].x), begin = __ldg(&p.sorted[first].x);
   const int prior = first > 0 ? __ldg(&p.sorted[first - 1].x) : -1;
@@ -419,7 +418,7 @@ __global__ void __launch_bounds__(kSumThreads) embed_join_kernel(SumParams p, G*
   int lo = piece + 1, hi = p.pieces - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(&p.sorted[mid * p.piece].x) == id) lo = mid;
+    if (__ldg(&p.sorted[mid * kPiece].x) == id) lo = mid;
     else hi = mid - 1;
   }
   const int stop = lo;
@@ -524,13 +523,11 @@ void embed_backward(const at::Tensor& ids, const at::Tensor& dout, double scale,
   }
   auto stream = at::cuda::getCurrentCUDAStream();
   SumParams p{};
-  // 32 tokens a CTA keep 148 SMs busy from 4736 tokens on; 64 halve the partials where there are plenty.
-  p.piece = n >= 16384 ? 64 : 32;
   p.n = static_cast<int>(n);
   p.V = V;
   p.H = static_cast<int>(H);
   p.scale = static_cast<float>(scale);
-  p.pieces = static_cast<int>((n + p.piece - 1) / p.piece);
+  p.pieces = static_cast<int>((n + kPiece - 1) / kPiece);
   // One workspace: partials, sorted pairs (twice and a histogram for many tokens), bitmap.
   const bool small = n <= kSmallMax;
   const int64_t tiles = (n + kSortTile - 1) / kSortTile;

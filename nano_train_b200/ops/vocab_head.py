@@ -32,6 +32,7 @@ from ._ext import ext
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 DEFAULT_WORKSPACE_MB = 2048
 MAX_TEACHER_LOGITS = 1024
+MAX_VOCAB = 1 << 19  # of a CUDA call (of a shard, with a group)
 
 
 def _world(group) -> int:
@@ -161,6 +162,8 @@ def _check(name, hidden, weight, reduction, max_workspace_mb):
             raise TypeError(f"{name}: CUDA tensors must be bfloat16, got {hidden.dtype}")
         if hidden.shape[-1] == 0 or hidden.shape[-1] % 8:
             raise ValueError(f"{name}: the hidden size must be a multiple of 8 on CUDA, got {hidden.shape[-1]}")
+        if weight.shape[0] > MAX_VOCAB:
+            raise ValueError(f"{name}: at most {MAX_VOCAB} words on CUDA, got {weight.shape[0]}")
 
 
 def _reduce(rows, valid, reduction):

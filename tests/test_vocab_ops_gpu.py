@@ -465,6 +465,8 @@ def test_refusals_on_cuda():
     with pytest.raises(ValueError):
         ops.linear_cross_entropy(h[:, :60], w[:, :60], lab)
     with pytest.raises(ValueError):
+        ops.linear_cross_entropy(h, w[:1].expand(2 ** 19 + 1, 64), lab)
+    with pytest.raises(ValueError):
         ops.linear_cross_entropy(h, w, lab[:7])
     with pytest.raises(ValueError):
         ops.linear_cross_entropy(h, w, lab.cpu())

@@ -45,6 +45,10 @@ namespace ntb {
 //     768 x 4096 with three, 0.84x at 4096^3 with three), so a split is taken only where the
 //     model saves more than 5 %.
 // Tensor-parallel ranks gain most: an N = 512 weight gradient is 64 wide tiles on 148 SMs.
+// The figures above are of the loops that one lane ran. Run by whole warps the narrow tile has nearly caught up
+// (4096^3: 108.6 us against 110.6 us of the wide single-CTA tile, 98.3 us of the pair), two slices of a 4096^3 weight
+// gradient no longer pay (107.4 against 106.5 us) and three still do at 768 x 4096 (38.9 against 45.1 us); the
+// constants are kept, so that every shape still takes the tiles it took.
 // NTB_GEMM_BN=128|256 forces the width; NTB_GEMM_SPLITK=0 turns the split off, =2..4 forces it.
 struct TileChoice {
   bool wide;
@@ -159,11 +163,11 @@ static void gemm_bf16_impl(const at::Tensor& a, const at::Tensor& b, at::Tensor&
     p.pub_ctr = pub_ctr;
     p.splits = 1;
   }
-  // CTA-pair tiles (256 x 256 on two SMs): measured 3-7 % faster than the single-CTA 128 x 256
-  // tile once each unit runs at least 2048 of K (4096^3: 107.5 against 113.7 us; 4096 x 4096 x
-  // 14336: 338.9 against 361.5 us; 4096^3 weight gradient in two K slices: 108.6 against 114.7 us)
-  // and up to 10 % slower on short K (K = 512: 44.0 against 39.9 us), where the pair's extra
-  // prologue is not amortised. NTB_GEMM_2SM=0 turns them off, =1 uses them for every wide tile.
+  // CTA-pair tiles (256 x 256 on two SMs): measured 8-13 % faster than the single-CTA 128 x 256 tile once each unit
+  // runs at least 2048 of K (4096^3: 98.3 against 110.6 us; 4096 x 4096 x 14336: 323.6 against 360.5 us; 4096 x 6144 x
+  // 4096: 140.3 against 151.6 us), about even at K = 1792 (54.2 against 56.2 us) and slower on short K (K = 512: 43.0
+  // against 41.0 us), where the pair's extra prologue is not amortised. NTB_GEMM_2SM=0 turns them off, =1 uses them
+  // for every wide tile.
   static const int pair_mode = [] {
     const char* e = std::getenv("NTB_GEMM_2SM");
     return e ? std::atoi(e) : -1;
